@@ -138,8 +138,9 @@ def _quantise(x, fmt, block):
     x = x.float().view(B, H, T // block, block * D)
     a = x.abs().amax(-1, keepdim=True)
     dead = ~(a >= TINY) | ~torch.isfinite(a)  # too small to divide by, or infinite or NaN: codes of 0
-    s = torch.where(dead, torch.where(a < TINY, 0.0, torch.nan), a / QMAX[fmt])
-    y = torch.where(dead, 0.0, x * (QMAX[fmt] / torch.where(dead, 1.0, a)))
+    top = torch.full_like(a, QMAX[fmt])  # a tensor: torch divides by, and takes the inverse of, a number in two roundings
+    s = torch.where(dead, torch.where(a < TINY, 0.0, torch.nan), a / top)
+    y = torch.where(dead, 0.0, x * (top / torch.where(dead, 1.0, a)))
     y = torch.round(y).to(torch.int8) if fmt == "int8" else y.to(torch.float8_e4m3fn)
     return y.view(B, H, T, D), s.squeeze(-1)
 
