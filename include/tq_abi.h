@@ -324,6 +324,88 @@ int tq_ragged_step(const tq_codec* kcodec, const tq_codec* vcodec, const void* k
                    const tq_store* vstore, int32_t batch, int32_t heads, const int32_t* seq_ints, int32_t n_ints,
                    int32_t* seq_ints_dev, void* stream);
 
+/* ---- 8-bit KV cache -----------------------------------------------------
+ * Keys and values of complete blocks of `block` tokens in 8 bits, one float32
+ * scale per (row, block) and side; the tokens of the last, incomplete block in
+ * kv_dtype. A sequence of n tokens has n - n % block tokens in codes and the
+ * other n % block in the tail, token p at tail slot p % block. For block
+ * elements x with a = max |x| and QMAX = 127 (int8) or 448 (e4m3):
+ *   scale = a / QMAX, code = round(x * (QMAX / a)), both in float32, codes to
+ *   the nearest (ties to even); a < 2^-110: scale 0, codes 0; a infinite or
+ *   NaN: scale NaN, codes 0 (the block reads back as NaN).
+ * Layouts: key codes (rows, cap, d); value codes in tiles of 64 tokens, each
+ * transposed, (rows, cap / 64, d, 64), so that the attention kernels load the
+ * operand of their second product as it is held; scales (rows, cap / block);
+ * tails (rows, block, d). rows = batch * heads. No counterpart in the
+ * reference, which keeps outlier layers in 16 bits (patch.py:337-338). */
+enum { TQ_KV8_INT8 = 0, TQ_KV8_E4M3 = 1 };
+
+typedef struct tq_kv8_store {
+  uint8_t* k_codes;      /* 16-byte aligned, like the other arrays but the scales */
+  uint8_t* v_codes;
+  float* k_scales;
+  float* v_scales;
+  void* k_tail;
+  void* v_tail;
+  int64_t cap;           /* tokens a row has room for: a multiple of 64, < 2^31 */
+  int32_t fmt;           /* TQ_KV8_* */
+  int32_t d;             /* 64, 96, 128 or 256 */
+  int32_t block;         /* 16, 32 or 64 */
+  int32_t kv_dtype;      /* TQ_F16 or TQ_BF16: tails, and the keys and values written */
+  int32_t batch, heads;
+} tq_kv8_store;
+
+/* Element (b, h, t, i) at p[b * sb + h * sh + t * st + i]; strides in elements,
+ * multiples of 8, p 16-byte aligned. */
+typedef struct tq_rows4 {
+  const void* p;
+  int64_t sb, sh, st;
+} tq_rows4;
+
+/* Writes tokens start .. start + n_new - 1 of every sequence from k, v
+ * (batch, heads, n_new, d) of kv_dtype: completed blocks are quantised (the
+ * first with what the tail holds of it), what is left goes to the tail.
+ * start_b / n_new_b: (batch,) device arrays, or NULL = start / n_new (which
+ * then bound them: start_b[b] + n_new_b[b] past cap and n_new_b[b] outside
+ * [0, n_new] write nothing for that sequence, nor does a negative start). */
+int tq_kv8_write(const tq_kv8_store* store, const tq_rows4* k, const tq_rows4* v, const int32_t* start_b, int32_t start,
+                 const int32_t* n_new_b, int32_t n_new, void* stream);
+
+/* Tokens start .. start + n - 1 of sequences of len_b[b] (or len) tokens, code
+ * * scale in float32 rounded once to out_dtype (any), to k_out and v_out
+ * (batch, heads, n, d), contiguous; tokens at or past a sequence's length
+ * give 0. */
+int tq_kv8_read(const tq_kv8_store* store, const int32_t* len_b, int32_t len, int32_t start, int32_t n,
+                int32_t out_dtype, void* k_out, void* v_out, void* stream);
+
+/* Attention of the last n_q tokens of every sequence over its cache: query i
+ * sits at position pos = len - n_q + i and sees the tokens t <= pos with
+ * t > pos - window or t < sinks (window 0: every t <= pos).
+ * out = softmax(scale q K^T) V, query head h reading kv head h / (hq / hkv);
+ * a query that sees nothing (pos < 0) gives 0. Scores, softmax and sums are in
+ * float32; the second product takes its weights in 16 bits. */
+typedef struct tq_kv_attn_desc {
+  int32_t batch, hq, hkv, d, n_q;
+  int32_t dtype;          /* TQ_F16 / TQ_BF16: q, and k, v (8-bit cache: == kv_dtype) */
+  int32_t out_dtype;      /* dtype or TQ_F32 */
+  int32_t window, sinks;
+  int32_t max_len;        /* bound of len_b (kernels clamp to it), or every length when NULL */
+  const int32_t* len_b;   /* (batch,) device, tokens per sequence, or NULL */
+  float scale;
+  tq_rows4 q;             /* (batch, hq, n_q, d) */
+  tq_rows4 out;           /* written, (batch, hq, n_q, d) */
+  tq_rows4 k, v;          /* tq_window_attention: (batch, hkv, >= max_len, d) */
+} tq_kv_attn_desc;
+
+/* Over an 8-bit cache (desc->k, v are not read), and over uncompressed keys
+ * and values of any strides. Workspace: scratch for the partials of one call,
+ * no initial contents; calls that share it must not overlap. */
+size_t tq_kv8_attention_workspace_bytes(const tq_kv8_store* store, const tq_kv_attn_desc* desc);
+int tq_kv8_attention(const tq_kv8_store* store, const tq_kv_attn_desc* desc, void* workspace, size_t workspace_bytes,
+                     void* stream);
+size_t tq_window_attention_workspace_bytes(const tq_kv_attn_desc* desc);
+int tq_window_attention(const tq_kv_attn_desc* desc, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

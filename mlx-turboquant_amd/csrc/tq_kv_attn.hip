@@ -1,0 +1,227 @@
+// Attention over 8-bit and uncompressed KV caches: checks, the split of the
+// tiles over workgroups, and the merge of the splits' partials.
+
+#include <math.h>
+
+#include "tq_kv8.h"
+
+namespace tq {
+namespace kv {
+
+int check_store(const tq_kv8_store* s);
+int check_rows(const tq_rows4& r, const char* what);
+
+extern template hipError_t launch_decode<64>(const Params&, bool, int, hipStream_t);
+extern template hipError_t launch_decode<96>(const Params&, bool, int, hipStream_t);
+extern template hipError_t launch_decode<128>(const Params&, bool, int, hipStream_t);
+extern template hipError_t launch_decode<256>(const Params&, bool, int, hipStream_t);
+extern template hipError_t launch_chunk<64>(const Params&, bool, int, hipStream_t);
+extern template hipError_t launch_chunk<96>(const Params&, bool, int, hipStream_t);
+extern template hipError_t launch_chunk<128>(const Params&, bool, int, hipStream_t);
+extern template hipError_t launch_chunk<256>(const Params&, bool, int, hipStream_t);
+
+namespace {
+
+constexpr int MT = 256;
+
+// One query row per workgroup: the partials (M, m, l, O) of its splits, O in
+// units of 2^M, l in units of 2^m, to out = 2^(M - m) O / l.
+template <int D, bool BF>
+__global__ __launch_bounds__(MT) void merge_kernel(const Params p, bool cached, int rows_per_tile) {
+  constexpr int L = D / 4, G = MT / L;  // lanes of 4 dims, groups of splits (D = 96: some threads idle)
+  __shared__ f4 os[G][L];
+  __shared__ float red[3][MT / 64];
+  const int unit = blockIdx.x;
+  const int bh = unit / p.rows, row = unit - bh * p.rows;
+  const int b = bh / p.hkv, h = bh - b * p.hkv;
+  const int qi = row / p.group, head = row - qi * p.group;
+  const int len = length_of(p, b);
+  const int r0 = row / rows_per_tile * rows_per_tile;
+  const int pmin = len - p.n_q + r0 / p.group, pmax = len - p.n_q + min(p.rows - 1, r0 + rows_per_tile - 1) / p.group;
+  const Tiles tl = tiles_of(len, cached, p.block_shift, pmin, pmax, p.window, p.sinks);
+  const int count = (tl.n + p.chunk - 1) / p.chunk;
+  const float* ml = p.ws + (int64_t)unit * p.splits * 4;
+
+  float M = -INFINITY, m = -INFINITY;
+  for (int i = threadIdx.x; i < count; i += MT) M = fmaxf(M, ml[4 * i]), m = fmaxf(m, ml[4 * i + 1]);
+  for (int k = 1; k < 64; k *= 2) M = fmaxf(M, __shfl_xor(M, k)), m = fmaxf(m, __shfl_xor(m, k));
+  if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = M, red[1][threadIdx.x >> 6] = m;
+  __syncthreads();
+  for (int k = 0; k < MT / 64; ++k) M = fmaxf(M, red[0][k]), m = fmaxf(m, red[1][k]);
+  const float Mr = M == -INFINITY ? 0.f : M, mr = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  for (int i = threadIdx.x; i < count; i += MT) l += ml[4 * i + 2] * __builtin_amdgcn_exp2f(ml[4 * i + 1] - mr);
+  for (int k = 1; k < 64; k *= 2) l += __shfl_xor(l, k);
+  if ((threadIdx.x & 63) == 0) red[2][threadIdx.x >> 6] = l;
+
+  const int c = threadIdx.x % L, grp = threadIdx.x / L;
+  f4 x = {0.f, 0.f, 0.f, 0.f};
+  if (grp < G) {
+    const float* o = p.ws + p.o_off + (int64_t)unit * p.splits * D + c * 4;
+    for (int i = grp; i < count; i += G) x += *(const f4*)(o + (int64_t)i * D) * __builtin_amdgcn_exp2f(ml[4 * i] - Mr);
+    os[grp][c] = x;
+  }
+  __syncthreads();
+  if (threadIdx.x >= L) return;
+  for (int i = 1; i < G; ++i) x += os[i][c];
+  l = 0.f;
+  for (int k = 0; k < MT / 64; ++k) l += red[2][k];
+  const float f = __builtin_amdgcn_exp2f(Mr - mr);
+  for (int k = 0; k < 4; ++k) x[k] = len - p.n_q + qi < 0 ? 0.f : x[k] / l * f;
+  const int64_t at = (int64_t)b * p.out.sb + (int64_t)(h * p.group + head) * p.out.sh + (int64_t)qi * p.out.st + c * 4;
+  if (p.out_f32)
+    *(f4*)((float*)p.out.p + at) = x;
+  else
+    *(u2*)((uint16_t*)p.out.p + at) = u2{bits2<BF>(x[0], x[1]), bits2<BF>(x[2], x[3])};
+}
+
+template <int D>
+hipError_t launch_merge(const Params& p, bool bf16, bool cached, int rows_per_tile, hipStream_t s) {
+  const uint32_t units = (uint32_t)(p.batch * p.hkv * p.rows);
+  if (bf16)
+    merge_kernel<D, true><<<units, MT, 0, s>>>(p, cached, rows_per_tile);
+  else
+    merge_kernel<D, false><<<units, MT, 0, s>>>(p, cached, rows_per_tile);
+  return hipGetLastError();
+}
+
+// Shapes of a call; fills what the launch needs but the pointers.
+int plan(const tq_kv8_store* s, const tq_kv_attn_desc* d, Params& p, bool& decode, size_t& bytes) {
+  if (d == nullptr) return set_error(TQ_ERR_INVALID, "attention: NULL descriptor");
+  if (d->d != 64 && d->d != 96 && d->d != 128 && d->d != 256)
+    return set_error(TQ_ERR_UNSUPPORTED, "attention: head_dim %d: use 64, 96, 128 or 256", d->d);
+  if (d->dtype != TQ_F16 && d->dtype != TQ_BF16) return set_error(TQ_ERR_UNSUPPORTED, "attention: fp16 or bf16 only");
+  if (d->out_dtype != d->dtype && d->out_dtype != TQ_F32)
+    return set_error(TQ_ERR_UNSUPPORTED, "attention: the output is of the queries' type or float32");
+  if (d->batch < 0 || d->hq < 1 || d->hkv < 1 || d->n_q < 0 || d->hq % d->hkv)
+    return set_error(TQ_ERR_INVALID, "attention: batch %d, %d query heads on %d, %d queries", d->batch, d->hq, d->hkv, d->n_q);
+  if (d->window < 0 || d->sinks < 0 || d->max_len < 0)
+    return set_error(TQ_ERR_INVALID, "attention: window %d, sinks %d, max_len %d", d->window, d->sinks, d->max_len);
+  if (d->max_len > 0x7fffffff - 4096 || d->n_q > 0x7fffffff - 4096 || (int64_t)d->n_q * (d->hq / d->hkv) > 0x7fffffff - 4096)
+    return set_error(TQ_ERR_UNSUPPORTED, "attention: too many tokens");
+  if (s != nullptr) {
+    if (int rc = check_store(s)) return rc;
+    if (s->d != d->d || s->batch != d->batch || s->heads != d->hkv || s->kv_dtype != d->dtype)
+      return set_error(TQ_ERR_INVALID, "attention: the cache is of other shapes or another type than the queries");
+    if (d->max_len > s->cap) return set_error(TQ_ERR_INVALID, "attention: length %d > the cache's room for %lld", d->max_len, (long long)s->cap);
+  }
+  p.batch = d->batch;
+  p.hkv = d->hkv;
+  p.group = d->hq / d->hkv;
+  p.n_q = d->n_q;
+  p.rows = p.group * p.n_q;
+  p.max_len = d->max_len;
+  p.block_shift = s == nullptr ? 0 : s->block == 16 ? 4 : s->block == 32 ? 5 : 6;
+  // a window of at least max_len hides nothing, and so no sinks matter
+  p.window = d->window >= d->max_len ? 0 : d->window;
+  p.sinks = p.window ? (d->sinks < d->max_len ? d->sinks : d->max_len) : 0;
+  p.out_f32 = d->out_dtype == TQ_F32;
+  p.scale = d->scale * 1.44269504088896340736f;
+  decode = p.rows <= DEC_ROWS;
+  p.row_tiles = decode ? 1 : (p.rows + CH_ROWS - 1) / CH_ROWS;
+
+  // tiles that a group of rows reads at most, the tail among them
+  int64_t tiles = ((int64_t)d->max_len + TILE - 1) / TILE;
+  if (p.window) {
+    const int64_t span = decode ? p.n_q : (p.n_q < CH_ROWS / p.group + 2 ? p.n_q : CH_ROWS / p.group + 2);
+    const int64_t w = (p.sinks + TILE - 1) / TILE + (p.window + span + TILE - 1) / TILE + 1;
+    tiles = w < tiles ? w : tiles;
+  }
+  tiles += s != nullptr;
+  if (tiles < 1) tiles = 1;
+  const int64_t base = (int64_t)p.batch * p.hkv * p.row_tiles;
+  int64_t splits = 1;
+  if (base > 0) {
+    const int64_t want = decode ? 1024 : 512;
+    splits = (want + base - 1) / base;
+    if (!decode && base >= 256) splits = 1;
+    const int64_t most = (tiles + 3) / 4;
+    if (splits > most) splits = most;
+    if (splits < 1) splits = 1;
+  }
+  int64_t chunk = (tiles + splits - 1) / splits;
+  if (decode) chunk = (chunk + DEC_WAVES - 1) / DEC_WAVES * DEC_WAVES;
+  splits = (tiles + chunk - 1) / chunk;
+  p.splits = (int)splits;
+  p.chunk = (int)chunk;
+  const int64_t units = (int64_t)p.batch * p.hkv * p.rows;
+  if (base * splits >= (int64_t)1 << 31 || units >= (int64_t)1 << 31)
+    return set_error(TQ_ERR_UNSUPPORTED, "attention: too many rows in one call");
+  p.o_off = units * splits * 4;
+  bytes = splits > 1 ? (size_t)(units * splits * (4 + d->d)) * sizeof(float) : 0;
+  return TQ_OK;
+}
+
+int attention(const tq_kv8_store* s, const tq_kv_attn_desc* d, void* ws, size_t ws_bytes, hipStream_t stream) {
+  Params p{};
+  bool decode;
+  size_t need;
+  if (int rc = plan(s, d, p, decode, need)) return rc;
+  if (p.batch == 0 || p.rows == 0) return TQ_OK;
+  if (int rc = check_rows(d->q, "attention: queries")) return rc;
+  if (int rc = check_rows(d->out, "attention: output")) return rc;
+  if (s == nullptr && d->max_len > 0) {
+    if (int rc = check_rows(d->k, "attention: keys")) return rc;
+    if (int rc = check_rows(d->v, "attention: values")) return rc;
+  }
+  if (need > 0 && (ws == nullptr || ws_bytes < need))
+    return set_error(TQ_ERR_WORKSPACE, "attention: workspace of %zu bytes, %zu needed", ws == nullptr ? (size_t)0 : ws_bytes, need);
+  if (need > 0 && ((uintptr_t)ws & 15)) return set_error(TQ_ERR_INVALID, "attention: the workspace needs 16-byte alignment");
+  p.q = {d->q.p, d->q.sb, d->q.sh, d->q.st};
+  p.out = {d->out.p, d->out.sb, d->out.sh, d->out.st};
+  p.k = {d->k.p, d->k.sb, d->k.sh, d->k.st};
+  p.v = {d->v.p, d->v.sb, d->v.sh, d->v.st};
+  p.len_b = d->len_b;
+  p.ws = (float*)ws;
+  int fmt = DENSE;
+  if (s != nullptr) {
+    fmt = s->fmt;
+    p.k_codes = s->k_codes;
+    p.v_codes = s->v_codes;
+    p.k_scales = s->k_scales;
+    p.v_scales = s->v_scales;
+    p.k_tail = (const uint16_t*)s->k_tail;
+    p.v_tail = (const uint16_t*)s->v_tail;
+    p.cap = s->cap;
+  }
+  const bool bf = d->dtype == TQ_BF16;
+  hipError_t e;
+  if (decode)
+    e = d->d == 64 ? launch_decode<64>(p, bf, fmt, stream) : d->d == 96 ? launch_decode<96>(p, bf, fmt, stream)
+        : d->d == 128 ? launch_decode<128>(p, bf, fmt, stream) : launch_decode<256>(p, bf, fmt, stream);
+  else
+    e = d->d == 64 ? launch_chunk<64>(p, bf, fmt, stream) : d->d == 96 ? launch_chunk<96>(p, bf, fmt, stream)
+        : d->d == 128 ? launch_chunk<128>(p, bf, fmt, stream) : launch_chunk<256>(p, bf, fmt, stream);
+  if (e == hipSuccess && p.splits > 1) {
+    const int rpt = decode ? p.rows : CH_ROWS;
+    const bool c = s != nullptr;
+    e = d->d == 64 ? launch_merge<64>(p, bf, c, rpt, stream) : d->d == 96 ? launch_merge<96>(p, bf, c, rpt, stream)
+        : d->d == 128 ? launch_merge<128>(p, bf, c, rpt, stream) : launch_merge<256>(p, bf, c, rpt, stream);
+  }
+  if (e != hipSuccess) return set_error(TQ_ERR_LAUNCH, "attention launch failed: %s", hipGetErrorString(e));
+  return TQ_OK;
+}
+
+size_t workspace(const tq_kv8_store* s, const tq_kv_attn_desc* d) {
+  Params p{};
+  bool decode;
+  size_t need = 0;
+  return plan(s, d, p, decode, need) == TQ_OK && p.batch > 0 && p.rows > 0 ? need : 0;
+}
+
+}  // namespace
+}  // namespace kv
+}  // namespace tq
+
+extern "C" size_t tq_kv8_attention_workspace_bytes(const tq_kv8_store* store, const tq_kv_attn_desc* desc) {
+  return store == nullptr ? 0 : tq::kv::workspace(store, desc);
+}
+extern "C" int tq_kv8_attention(const tq_kv8_store* store, const tq_kv_attn_desc* desc, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+  if (store == nullptr) return tq::set_error(TQ_ERR_INVALID, "kv8: NULL store");
+  return tq::kv::attention(store, desc, workspace, workspace_bytes, (hipStream_t)stream);
+}
+extern "C" size_t tq_window_attention_workspace_bytes(const tq_kv_attn_desc* desc) { return tq::kv::workspace(nullptr, desc); }
+extern "C" int tq_window_attention(const tq_kv_attn_desc* desc, void* workspace, size_t workspace_bytes, void* stream) {
+  return tq::kv::attention(nullptr, desc, workspace, workspace_bytes, (hipStream_t)stream);
+}

@@ -72,7 +72,28 @@ class AttnDesc(ctypes.Structure):
 
 TQ_ATTN_GENERAL = 1
 
+TQ_KV8_INT8, TQ_KV8_E4M3 = 0, 1
 
+
+class KV8StoreDesc(ctypes.Structure):
+    _fields_ = [("k_codes", _p), ("v_codes", _p), ("k_scales", _p), ("v_scales", _p), ("k_tail", _p), ("v_tail", _p),
+                ("cap", _i64), ("fmt", _i32), ("d", _i32), ("block", _i32), ("kv_dtype", _i32),
+                ("batch", _i32), ("heads", _i32)]
+
+
+class Rows4(ctypes.Structure):
+    _fields_ = [("p", _p), ("sb", _i64), ("sh", _i64), ("st", _i64)]
+
+
+class KVAttnDesc(ctypes.Structure):
+    _fields_ = [("batch", _i32), ("hq", _i32), ("hkv", _i32), ("d", _i32), ("n_q", _i32),
+                ("dtype", _i32), ("out_dtype", _i32), ("window", _i32), ("sinks", _i32), ("max_len", _i32),
+                ("len_b", _p), ("scale", ctypes.c_float), ("q", Rows4), ("out", Rows4), ("k", Rows4), ("v", Rows4)]
+
+
+_P8 = ctypes.POINTER(KV8StoreDesc)
+_PR = ctypes.POINTER(Rows4)
+_PK = ctypes.POINTER(KVAttnDesc)
 _PC = ctypes.POINTER(Codec)
 _PS = ctypes.POINTER(Store)
 _PSp = ctypes.POINTER(Span)
@@ -101,6 +122,12 @@ SIGNATURES = {
     "tq_decode_attention_noalloc": (_i32, [_PC, _PC, _PA, _p]),
     "tq_dense_decode_workspace_bytes": (ctypes.c_size_t, [_PA, _i32]),
     "tq_dense_decode_attention": (_i32, [_PA, _i32, _p, ctypes.c_size_t, _p]),
+    "tq_kv8_write": (_i32, [_P8, _PR, _PR, _p, _i32, _p, _i32, _p]),
+    "tq_kv8_read": (_i32, [_P8, _p, _i32, _i32, _i32, _i32, _p, _p, _p]),
+    "tq_kv8_attention_workspace_bytes": (ctypes.c_size_t, [_P8, _PK]),
+    "tq_kv8_attention": (_i32, [_P8, _PK, _p, ctypes.c_size_t, _p]),
+    "tq_window_attention_workspace_bytes": (ctypes.c_size_t, [_PK]),
+    "tq_window_attention": (_i32, [_PK, _p, ctypes.c_size_t, _p]),
 }
 
 _lib = None
