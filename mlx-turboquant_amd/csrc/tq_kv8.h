@@ -3,6 +3,8 @@
 // list of 64-token tiles a group of queries has to read.
 #pragma once
 
+#include <math.h>
+
 #include "tq_common.h"
 
 namespace tq {
@@ -19,6 +21,7 @@ typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int TILE = 64;     // tokens per tile (and per transposed tile of value codes)
+constexpr int HALF = TILE / 2;
 constexpr int DEC_WAVES = 4, DEC_ROWS = 16;            // tq_kv_decode.h: waves and most rows per workgroup
 constexpr int CH_WAVES = 4, CH_ROWS = CH_WAVES * 32;   // tq_kv_chunk.h
 constexpr int DENSE = -1;    // format of uncompressed keys and values (else TQ_KV8_*)
@@ -86,6 +89,53 @@ __device__ inline uint32_t bits2(float a, float b) {
     return __builtin_bit_cast(uint32_t, h2{(_Float16)a, (_Float16)b});
 }
 
+// Values that are infinite or NaN, in tiles that some rows see only in part:
+// taken out of the product (0 x inf would reach the rows that do not see them)
+// and counted in one of their own, marks x seen: 1 for inf, 128 for -inf, 2^14
+// for NaN (at most 64 of each per tile: exact), which gives back what the rows
+// that see them get.
+// Bits 15 and 31: the exponent of that half is all ones (adding one to it carries).
+template <bool BF>
+__device__ inline uint32_t odd16(uint32_t x) {
+  return (x & 0x7fff7fffu) + (BF ? 0x00800080u : 0x04000400u);
+}
+constexpr uint32_t ODD_BITS = 0x80008000u;
+template <bool BF>
+__device__ inline uint32_t mark16(uint32_t h) {
+  constexpr uint32_t ex = BF ? 0x7f80u : 0x7c00u;
+  if ((h & ex) != ex) return 0u;
+  if (h & 0x7fffu & ~ex) return BF ? 0x4680u : 0x7400u;  // 16384
+  return h & 0x8000u ? (BF ? 0x4300u : 0x5800u) : (BF ? 0x3f80u : 0x3c00u);  // 128, 1
+}
+template <bool BF>
+__device__ inline u4 marks(u4& v) {
+  u4 m;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = mark16<BF>(v[i] & 0xffffu), hi = mark16<BF>(v[i] >> 16);
+    m[i] = lo | hi << 16;
+    v[i] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+  }
+  return m;
+}
+__device__ inline float marked(float c) {
+  const uint32_t n = (uint32_t)c;
+  const float up = n & 127u ? INFINITY : 0.f, down = n & 127u << 7 ? -INFINITY : 0.f;
+  return n >> 14 ? NAN : up + down;
+}
+// Bit i: the row at position pos sees token t + i (i < count <= 16): t + i <
+// end, <= pos, and > low or < sinks.
+__device__ inline uint32_t seen_bits(int t, int count, int end, int pos, int low, int sinks) {
+  const auto below = [&](int x) { return (1u << min(max(x - t, 0), count)) - 1u; };  // tokens before x
+  return below(min(end, pos + 1)) & (~below(low + 1) | below(sinks));
+}
+// 1.0 in the halves whose token is seen (bits 0 and 1)
+template <bool BF>
+__device__ inline uint32_t seen2(uint32_t bits) {
+  constexpr uint32_t one = BF ? 0x3f80u : 0x3c00u;
+  return (bits & 1u ? one : 0u) | (bits & 2u ? one << 16 : 0u);
+}
+
 template <bool BF>
 __device__ inline f4 mma16(u4 a, u4 b, f4 c) {
   if constexpr (BF)
@@ -101,6 +151,20 @@ __device__ inline f16v mma32(u4 a, u4 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
 
+// The maximum over the lanes that differ in bits 4 and 5 (16) or 5 (32)
+// of their number, without a trip through LDS.
+template <int FROM>
+__device__ inline float lanes_max(float x) {
+  uint32_t v = __float_as_uint(x);
+  if constexpr (FROM == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    v = __float_as_uint(x);
+  }
+  const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 // Rows of an operand: element (b, h, t, i) at p[b * sb + h * sh + t * st + i].
 struct Rows {
   const void* p;
@@ -114,12 +178,13 @@ struct Params {
   const uint16_t *k_tail, *v_tail;
   int64_t cap;
   const int32_t* len_b;
-  float* ws;              // partials: ML (units, splits, 4), then O (units, splits, D)
+  float* ws;              // partials: (M, m, l, -) per slot, then O (slots, D)
   int64_t o_off;          // floats before the O part
   int32_t batch, hkv, group, n_q, rows;  // rows = group * n_q per kv head, row = i * group + head
   int32_t max_len, block_shift, window, sinks;
-  int32_t splits, chunk;  // a split is `chunk` consecutive tiles
-  int32_t row_tiles;      // row tiles of a kv head (chunk kernel)
+  int32_t wgs;            // decode: workgroups that share the list of all tiles; 0: one per (sequence, kv head)
+  int32_t splits, chunk;  // chunk kernel: a split is `chunk` consecutive tiles
+  int32_t row_tiles;      // chunk kernel: row tiles of a kv head
   int32_t out_f32;
   float scale;            // times log2 e: scores are kept in base 2
 };
@@ -150,6 +215,82 @@ __device__ inline Tiles tiles_of(int len, bool cached, int block_shift, int pmin
 
 __device__ inline int length_of(const Params& p, int b) {
   return p.len_b ? min(max(p.len_b[b], 0), p.max_len) : p.max_len;
+}
+
+// Decode's list of tiles: those of (sequence 0, kv head 0), (0, 1), ... Each of
+// p.wgs workgroups takes `per` consecutive ones, whatever sequences they belong
+// to, so that sequences of any lengths load the chip evenly. The part of
+// (sequence, kv head) unit u that workgroup w holds goes to partial slot w + u:
+// along the list each step is to the next w or the next u, so slots are distinct.
+// In the list a unit's tiles are filled up to a multiple of DEC_WAVES (places
+// without a tile): as many as its waves take at once, so that short shares hold
+// no parts of two units, which would take twice as long.
+struct Share {
+  int total, per;   // places in the list, places per workgroup
+};
+
+__device__ inline int decode_places(const Params& p, bool cached, int b) {
+  const int len = length_of(p, b);
+  const int n = tiles_of(len, cached, p.block_shift, len - p.n_q, len - 1, p.window, p.sinks).n;
+  return (n + DEC_WAVES - 1) / DEC_WAVES * DEC_WAVES;
+}
+
+// Inclusive sums over the wave's lanes.
+__device__ inline int wave_scan(int n, int lane) {
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) {
+    const int up = __shfl_up(n, k);
+    if (lane >= k) n += up;
+  }
+  return n;
+}
+
+// The share, and for workgroup `wg` (>= 0) the sequence that its first tile
+// belongs to (b; -1: no tiles) or for sequence b: the tiles before it.
+__device__ inline Share share_of(const Params& p, bool cached, int wg, int& b, int& before) {
+  const int lane = threadIdx.x & 63;
+  Share s;
+  const auto per_of = [&](int total) {
+    s.total = total;
+    s.per = max(DEC_WAVES, ((total + p.wgs - 1) / p.wgs + DEC_WAVES - 1) / DEC_WAVES * DEC_WAVES);
+  };
+  if (p.len_b == nullptr) {
+    const int n = decode_places(p, cached, 0) * p.hkv;
+    per_of(n * p.batch);
+    if (wg >= 0) b = wg * s.per < s.total ? wg * s.per / n : -1;
+    before = b * n;
+    return s;
+  }
+  int n = lane < p.batch ? decode_places(p, cached, lane) * p.hkv : 0;
+  int sum = wave_scan(n, lane);  // of the first 64 sequences
+  int total = __shfl(sum, 63);
+  for (int b0 = 64; b0 < p.batch; b0 += 64)
+    total += __shfl(wave_scan(b0 + lane < p.batch ? decode_places(p, cached, b0 + lane) * p.hkv : 0, lane), 63);
+  per_of(__builtin_amdgcn_readfirstlane(total));
+  const int at = wg * s.per;
+  if (wg >= 0 && at >= s.total) {
+    b = -1;
+    return s;
+  }
+  int base = 0;
+  for (int b0 = 0;; b0 += 64) {
+    int l = -1;
+    if (wg >= 0) {
+      const uint64_t past = __ballot(base + sum > at);
+      if (past) l = __builtin_ctzll(past);
+    } else if (b < b0 + 64) {
+      l = b - b0;
+    }
+    if (l >= 0) {
+      if (l > 0) base += __shfl(sum, l - 1);
+      before = __builtin_amdgcn_readfirstlane(base);
+      b = __builtin_amdgcn_readfirstlane(b0 + l);
+      return s;
+    }
+    base += __shfl(sum, 63);
+    n = b0 + 64 + lane < p.batch ? decode_places(p, cached, b0 + 64 + lane) * p.hkv : 0;
+    sum = wave_scan(n, lane);
+  }
 }
 
 // Kernels by head dim (one source file each): FMT of DENSE / TQ_KV8_*.

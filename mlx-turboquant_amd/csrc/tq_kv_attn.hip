@@ -3,6 +3,8 @@
 
 #include <math.h>
 
+#include <algorithm>
+
 #include "tq_kv8.h"
 
 namespace tq {
@@ -23,11 +25,16 @@ extern template hipError_t launch_chunk<256>(const Params&, bool, int, hipStream
 namespace {
 
 constexpr int MT = 256;
+// Up to so many tiles, one workgroup per (sequence, kv head) and no merge.
+constexpr int DIRECT_TILES = 12;
+// Workgroups that share the tiles otherwise: two per CU, what their registers
+// allow.
+constexpr int STREAM_WGS = 512;
 
 // One query row per workgroup: the partials (M, m, l, O) of its splits, O in
 // units of 2^M, l in units of 2^m, to out = 2^(M - m) O / l.
 template <int D, bool BF>
-__global__ __launch_bounds__(MT) void merge_kernel(const Params p, bool cached, int rows_per_tile) {
+__global__ __launch_bounds__(MT) void merge_kernel(const Params p, bool cached) {
   constexpr int L = D / 4, G = MT / L;  // lanes of 4 dims, groups of splits (D = 96: some threads idle)
   __shared__ f4 os[G][L];
   __shared__ float red[3][MT / 64];
@@ -36,29 +43,42 @@ __global__ __launch_bounds__(MT) void merge_kernel(const Params p, bool cached, 
   const int b = bh / p.hkv, h = bh - b * p.hkv;
   const int qi = row / p.group, head = row - qi * p.group;
   const int len = length_of(p, b);
-  const int r0 = row / rows_per_tile * rows_per_tile;
-  const int pmin = len - p.n_q + r0 / p.group, pmax = len - p.n_q + min(p.rows - 1, r0 + rows_per_tile - 1) / p.group;
-  const Tiles tl = tiles_of(len, cached, p.block_shift, pmin, pmax, p.window, p.sinks);
-  const int count = (tl.n + p.chunk - 1) / p.chunk;
-  const float* ml = p.ws + (int64_t)unit * p.splits * 4;
+  int count;
+  int64_t slot, step;  // first partial, distance of the next
+  if (p.wgs) {
+    int seq = b, before;
+    const Share sh = share_of(p, cached, -1, seq, before);
+    const int n = decode_places(p, cached, b), at = before + h * n;
+    count = n ? (at + n - 1) / sh.per - at / sh.per + 1 : 0;
+    slot = (int64_t)(at / sh.per + bh) * p.rows + row;
+    step = p.rows;
+  } else {
+    const int r0 = row / CH_ROWS * CH_ROWS;
+    const int pmin = len - p.n_q + r0 / p.group, pmax = len - p.n_q + min(p.rows - 1, r0 + CH_ROWS - 1) / p.group;
+    count = (tiles_of(len, cached, p.block_shift, pmin, pmax, p.window, p.sinks).n + p.chunk - 1) / p.chunk;
+    slot = (int64_t)unit * p.splits;
+    step = 1;
+  }
+  const float* ml = p.ws + slot * 4;
+  step *= 4;
 
   float M = -INFINITY, m = -INFINITY;
-  for (int i = threadIdx.x; i < count; i += MT) M = fmaxf(M, ml[4 * i]), m = fmaxf(m, ml[4 * i + 1]);
+  for (int i = threadIdx.x; i < count; i += MT) M = fmaxf(M, ml[step * i]), m = fmaxf(m, ml[step * i + 1]);
   for (int k = 1; k < 64; k *= 2) M = fmaxf(M, __shfl_xor(M, k)), m = fmaxf(m, __shfl_xor(m, k));
   if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = M, red[1][threadIdx.x >> 6] = m;
   __syncthreads();
   for (int k = 0; k < MT / 64; ++k) M = fmaxf(M, red[0][k]), m = fmaxf(m, red[1][k]);
   const float Mr = M == -INFINITY ? 0.f : M, mr = m == -INFINITY ? 0.f : m;
   float l = 0.f;
-  for (int i = threadIdx.x; i < count; i += MT) l += ml[4 * i + 2] * __builtin_amdgcn_exp2f(ml[4 * i + 1] - mr);
+  for (int i = threadIdx.x; i < count; i += MT) l += ml[step * i + 2] * __builtin_amdgcn_exp2f(ml[step * i + 1] - mr);
   for (int k = 1; k < 64; k *= 2) l += __shfl_xor(l, k);
   if ((threadIdx.x & 63) == 0) red[2][threadIdx.x >> 6] = l;
 
   const int c = threadIdx.x % L, grp = threadIdx.x / L;
   f4 x = {0.f, 0.f, 0.f, 0.f};
   if (grp < G) {
-    const float* o = p.ws + p.o_off + (int64_t)unit * p.splits * D + c * 4;
-    for (int i = grp; i < count; i += G) x += *(const f4*)(o + (int64_t)i * D) * __builtin_amdgcn_exp2f(ml[4 * i] - Mr);
+    const float* o = p.ws + p.o_off + slot * D + c * 4;
+    for (int i = grp; i < count; i += G) x += *(const f4*)(o + step / 4 * i * D) * __builtin_amdgcn_exp2f(ml[step * i] - Mr);
     os[grp][c] = x;
   }
   __syncthreads();
@@ -76,12 +96,12 @@ __global__ __launch_bounds__(MT) void merge_kernel(const Params p, bool cached, 
 }
 
 template <int D>
-hipError_t launch_merge(const Params& p, bool bf16, bool cached, int rows_per_tile, hipStream_t s) {
+hipError_t launch_merge(const Params& p, bool bf16, bool cached, hipStream_t s) {
   const uint32_t units = (uint32_t)(p.batch * p.hkv * p.rows);
   if (bf16)
-    merge_kernel<D, true><<<units, MT, 0, s>>>(p, cached, rows_per_tile);
+    merge_kernel<D, true><<<units, MT, 0, s>>>(p, cached);
   else
-    merge_kernel<D, false><<<units, MT, 0, s>>>(p, cached, rows_per_tile);
+    merge_kernel<D, false><<<units, MT, 0, s>>>(p, cached);
   return hipGetLastError();
 }
 
@@ -129,26 +149,25 @@ int plan(const tq_kv8_store* s, const tq_kv_attn_desc* d, Params& p, bool& decod
   }
   tiles += s != nullptr;
   if (tiles < 1) tiles = 1;
-  const int64_t base = (int64_t)p.batch * p.hkv * p.row_tiles;
-  int64_t splits = 1;
-  if (base > 0) {
-    const int64_t want = decode ? 1024 : 512;
-    splits = (want + base - 1) / base;
-    if (!decode && base >= 256) splits = 1;
+  const int64_t units = (int64_t)p.batch * p.hkv, base = units * p.row_tiles;
+  if (base >= (int64_t)1 << 31 || units * p.rows >= (int64_t)1 << 31 || units * tiles >= (int64_t)1 << 30)
+    return set_error(TQ_ERR_UNSUPPORTED, "attention: too many rows or tokens in one call");
+  int64_t slots = 0;
+  if (decode) {
+    p.wgs = 0;
+    if (tiles > DIRECT_TILES) p.wgs = (int)std::min<int64_t>(STREAM_WGS, units * ((tiles + DEC_WAVES - 1) / DEC_WAVES));
+    if (p.wgs) slots = (p.wgs + units) * p.rows;
+  } else {
+    int64_t splits = base > 0 && base < 256 ? (512 + base - 1) / base : 1;
     const int64_t most = (tiles + 3) / 4;
     if (splits > most) splits = most;
-    if (splits < 1) splits = 1;
+    p.chunk = (int)((tiles + splits - 1) / splits);
+    p.splits = (int)((tiles + p.chunk - 1) / p.chunk);
+    if (base * p.splits >= (int64_t)1 << 31) return set_error(TQ_ERR_UNSUPPORTED, "attention: too many rows in one call");
+    if (p.splits > 1) slots = units * p.rows * p.splits;
   }
-  int64_t chunk = (tiles + splits - 1) / splits;
-  if (decode) chunk = (chunk + DEC_WAVES - 1) / DEC_WAVES * DEC_WAVES;
-  splits = (tiles + chunk - 1) / chunk;
-  p.splits = (int)splits;
-  p.chunk = (int)chunk;
-  const int64_t units = (int64_t)p.batch * p.hkv * p.rows;
-  if (base * splits >= (int64_t)1 << 31 || units >= (int64_t)1 << 31)
-    return set_error(TQ_ERR_UNSUPPORTED, "attention: too many rows in one call");
-  p.o_off = units * splits * 4;
-  bytes = splits > 1 ? (size_t)(units * splits * (4 + d->d)) * sizeof(float) : 0;
+  p.o_off = slots * 4;
+  bytes = (size_t)(slots * (4 + d->d)) * sizeof(float);
   return TQ_OK;
 }
 
@@ -192,11 +211,10 @@ int attention(const tq_kv8_store* s, const tq_kv_attn_desc* d, void* ws, size_t 
   else
     e = d->d == 64 ? launch_chunk<64>(p, bf, fmt, stream) : d->d == 96 ? launch_chunk<96>(p, bf, fmt, stream)
         : d->d == 128 ? launch_chunk<128>(p, bf, fmt, stream) : launch_chunk<256>(p, bf, fmt, stream);
-  if (e == hipSuccess && p.splits > 1) {
-    const int rpt = decode ? p.rows : CH_ROWS;
+  if (e == hipSuccess && need > 0) {
     const bool c = s != nullptr;
-    e = d->d == 64 ? launch_merge<64>(p, bf, c, rpt, stream) : d->d == 96 ? launch_merge<96>(p, bf, c, rpt, stream)
-        : d->d == 128 ? launch_merge<128>(p, bf, c, rpt, stream) : launch_merge<256>(p, bf, c, rpt, stream);
+    e = d->d == 64 ? launch_merge<64>(p, bf, c, stream) : d->d == 96 ? launch_merge<96>(p, bf, c, stream)
+        : d->d == 128 ? launch_merge<128>(p, bf, c, stream) : launch_merge<256>(p, bf, c, stream);
   }
   if (e != hipSuccess) return set_error(TQ_ERR_LAUNCH, "attention launch failed: %s", hipGetErrorString(e));
   return TQ_OK;

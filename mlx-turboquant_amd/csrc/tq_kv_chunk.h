@@ -18,8 +18,8 @@
 // is below 2^-17 (then off by at most 2^-25, half the smallest fp16).
 // Both are the same for 16 tokens, so uniform over a wave.
 //
-// A value that is infinite or NaN in a tile that some rows see only in part
-// would reach the rows that do not see it (0 x inf): then row by row.
+// Infinite and NaN values in 16-bit tiles that some rows see only in part are
+// taken apart (marks()).
 #pragma once
 
 #include <math.h>
@@ -87,7 +87,7 @@ struct Chunk {
       if (t < nv) x = *(const u4*)(kb + (int64_t)t * kst + c * 8);
       *(u4*)(kl + krow(t) * KP + c * 8) = x;
     }
-    bool odd = false;
+    uint32_t odd = 0;
     // 4 tokens x 8 dims per thread, paired by tokens
     for (int i = threadIdx.x; i < TILE / 4 * (D / 8); i += CH_THREADS) {
       const int c = i % (D / 8), t = i / (D / 8) * 4;
@@ -96,9 +96,8 @@ struct Chunk {
       for (int u = 0; u < 4; ++u) {
         x[u] = u4{0, 0, 0, 0};
         if (t + u < nv) x[u] = *(const u4*)(vb + (int64_t)(t + u) * vst + c * 8);
-        const uint32_t ex = BF ? 0x7f80u : 0x7c00u;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) odd |= (x[u][k] & ex) == ex || (x[u][k] & ex << 16) == ex << 16;
+        for (int k = 0; k < 4; ++k) odd |= odd16<BF>(x[u][k]);
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -107,7 +106,7 @@ struct Chunk {
             u2{__builtin_amdgcn_perm(x[1][k / 2], x[0][k / 2], sel), __builtin_amdgcn_perm(x[3][k / 2], x[2][k / 2], sel)};
       }
     }
-    return odd;
+    return odd & ODD_BITS;
   }
 };
 
@@ -137,7 +136,7 @@ __global__ __launch_bounds__(CH_THREADS, D > 128 ? 1 : 2) void chunk_kernel(cons
   const int first = split * p.chunk, last = min(tl.n, first + p.chunk);
   if (p.splits > 1 && first >= tl.n) return;  // the merge kernel counts the same tiles
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, hf = lane >> 5;
   const int row = row0 + wave * 32 + n;
   const bool live = row < p.rows;
@@ -221,14 +220,17 @@ __global__ __launch_bounds__(CH_THREADS, D > 128 ? 1 : 2) void chunk_kernel(cons
       for (int k = 0; k < 8; ++k) s[grp >> 1][(grp & 1) * 8 + k] *= c;
     }
     const bool masked = nv < TILE || t0 + TILE - 1 > wpmin || (p.window && t0 <= wpmax - p.window && t0 + TILE > p.sinks);
+    uint32_t seen[4];
     if (masked) {
 #pragma unroll
-      for (int grp = 0; grp < 4; ++grp)
+      for (int grp = 0; grp < 4; ++grp) {
+        seen[grp] = seen_bits(t0 + 16 * grp + 8 * hf, 8, t0 + nv, pos, low, p.sinks);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const int i = 16 * grp + 8 * hf + k, t = t0 + i;
-          if (!(i < nv && t <= pos && (t > low || t < p.sinks))) s[grp >> 1][(grp & 1) * 8 + k] = -INFINITY;
+          const float x = s[grp >> 1][(grp & 1) * 8 + k];
+          s[grp >> 1][(grp & 1) * 8 + k] = seen[grp] >> k & 1 ? x : -INFINITY;
         }
+      }
     }
     // softmax
     float top = -INFINITY;
@@ -236,7 +238,7 @@ __global__ __launch_bounds__(CH_THREADS, D > 128 ? 1 : 2) void chunk_kernel(cons
     for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
       for (int k = 0; k < 16; ++k) top = fmaxf(top, s[sub][k]);
-    top = fmaxf(top, __shfl_xor(top, 32));
+    top = lanes_max<32>(top);
     const float mn = fmaxf(m, top - W_SHIFT);
     const float ref = mn == -INFINITY ? 0.f : mn;
     if (__any(mn > m)) {
@@ -269,25 +271,21 @@ __global__ __launch_bounds__(CH_THREADS, D > 128 ? 1 : 2) void chunk_kernel(cons
     if (masked && odd_tile) {
 #pragma unroll
       for (int i = 0; i < NO; ++i) {
-#pragma unroll 1
-        for (int r = 0; r < 32; ++r) {
-          const int at = __shfl(pos, r), lw = __shfl(low, r);
-          f16v x;
+        const uint16_t* vp = vl + (i * 32 + n) * C::VP + hf * 8;
+        f16v x;
 #pragma unroll
-          for (int k = 0; k < 16; ++k) x[k] = 0.f;
+        for (int k = 0; k < 16; ++k) x[k] = 0.f;
 #pragma unroll
-          for (int grp = 0; grp < 4; ++grp) {
-            u4 v = *(const u4*)(vl + (i * 32 + n) * C::VP + grp * 16 + hf * 8);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int k = 16 * grp + 8 * hf + 2 * u, t = t0 + k;
-              const bool a = t <= at && (t > lw || t < p.sinks), c = t + 1 <= at && (t + 1 > lw || t + 1 < p.sinks);
-              v[u] &= (a ? 0xffffu : 0u) | (c ? 0xffff0000u : 0u);
-            }
-            x = mma32<BF>(v, pw[grp], x);
-          }
-          o[i] = n == r ? o[i] + x : o[i];
+        for (int grp = 0; grp < 4; ++grp) {
+          u4 v = *(const u4*)(vp + grp * 16);
+          const u4 ones = {seen2<BF>(seen[grp]), seen2<BF>(seen[grp] >> 2), seen2<BF>(seen[grp] >> 4), seen2<BF>(seen[grp] >> 6)};
+          x = mma32<BF>(marks<BF>(v), ones, x);
+          o[i] = mma32<BF>(v, pw[grp], o[i]);
+          __builtin_amdgcn_sched_barrier(0);  // one at a time: this is rare, registers are not
         }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o[i][k] += marked(x[k]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     } else {
 #pragma unroll

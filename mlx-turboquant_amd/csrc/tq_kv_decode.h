@@ -24,9 +24,8 @@
 // exp2(s - m) has its own maximum m. 16-bit tiles of bf16 take the weights as
 // two bf16 parts.
 //
-// Masked scores are -inf and their weights 0. In 16-bit tiles that some rows
-// see only in part, a value that is infinite or NaN would reach the rows that
-// do not see it (0 x inf): such tiles are done row by row.
+// Masked scores are -inf and their weights 0; infinite and NaN values in 16-bit
+// tiles that some rows see only in part are taken apart (marks()).
 #pragma once
 
 #include <math.h>
@@ -43,6 +42,7 @@ struct Decode {
   static constexpr int NO = D / 16;   // 16-dim tiles of the output
   static constexpr int NC = D / 64;   // 64-byte pieces of a code row
   static constexpr bool ODD = D % 64 != 0;
+  static constexpr bool AHEAD = D <= 128;
 
   const Params& p;
   int n, g;           // query row (column of S^T), lane group
@@ -60,7 +60,6 @@ struct Decode {
     if (!CACHED) return st * 32 + gg * 8;
     return st < 2 * NC ? (st >> 1) * 64 + gg * 16 + (st & 1) * 8 : NC * 64 + gg * 8;
   }
-  __device__ bool sees(int t, int at, int lw) const { return t <= at && (t > lw || t < p.sinks); }
 
   __device__ void load_q(const uint16_t* qp, bool live, u4 (&f)[NS]) const {
 #pragma unroll
@@ -77,8 +76,7 @@ struct Decode {
         top = fmaxf(top, fabsf(elem<true>(f[st][i] & 0xffff)));
         top = fmaxf(top, fabsf(elem<true>(f[st][i] >> 16)));
       }
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
+    top = lanes_max<16>(top);
     int e = 0;
     if (top > 0.f && top < INFINITY) e = 15 - (ilogbf(top) + 1);
 #pragma unroll
@@ -90,15 +88,12 @@ struct Decode {
   }
 
   // Scores (masked: -inf) to weights, and the running maxima and sum.
-  template <bool TWO>
-  __device__ void weights(const float (&s)[16], float lv, bool masked, float (&w)[16]) {
+  template <bool TWO, int N>
+  __device__ void weights(const float (&s)[N], float lv, bool masked, float (&w)[N]) {
     float mx = s[0];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-    float top = TWO ? mx + lv : mx;
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const float Mn = fmaxf(M, top - W_SHIFT);
+    for (int i = 1; i < N; ++i) mx = fmaxf(mx, s[i]);
+    const float Mn = fmaxf(M, lanes_max<16>(TWO ? mx + lv : mx) - W_SHIFT);
     const float ref = Mn == -INFINITY ? 0.f : Mn;
     if (__any(Mn > M)) {
       const float a = __builtin_amdgcn_exp2f(M - ref);
@@ -107,52 +102,69 @@ struct Decode {
       if (!TWO) l *= a;
       M = Mn;
     }
-    const float off = TWO ? lv - ref : -ref;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = __builtin_amdgcn_exp2f(s[i] + off);
-    if (masked) {  // a block without a finite scale is NaN where it is seen only
-#pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = s[i] == -INFINITY ? 0.f : w[i];
-    }
+    // one exponential per score, against the lane's own largest of the tile
+    // where two references are needed: both are then a factor
+    const float near = TWO ? (mx == -INFINITY ? 0.f : mx) : ref;
     float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      w[i] = __builtin_amdgcn_exp2f(s[i] - near);
+      sum += w[i];
+    }
     if (TWO) {
-      const float mn = fmaxf(m, mx);
+      const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(mx + lv - ref);
       const float mref = mn == -INFINITY ? 0.f : mn;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sum += __builtin_amdgcn_exp2f(s[i] - mref);
-      l = l * __builtin_amdgcn_exp2f(m - mref) + sum;
+      l = l * __builtin_amdgcn_exp2f(m - mref) + sum * __builtin_amdgcn_exp2f(mx - mref);
       m = mn;
-    } else {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sum += w[i];
+      for (int i = 0; i < N; ++i) w[i] *= f;
+    } else {
       l += sum;
+    }
+    if (TWO && masked) {  // a block without a finite scale is NaN where it is seen only
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[i] = s[i] == -INFINITY ? 0.f : w[i];
     }
   }
 
-  // Whether every row sees all of tokens t0 .. t0 + 63.
-  __device__ bool whole(int t0, int len) const {
-    return t0 + TILE <= len && t0 + TILE - 1 <= pmin && (t0 > lowmax || t0 + TILE <= p.sinks);
+  // Whether every row sees all of tokens t0 .. t0 + count - 1.
+  __device__ bool whole(int t0, int count, int len) const {
+    return t0 + count <= len && t0 + count - 1 <= pmin && (t0 > lowmax || t0 + count <= p.sinks);
   }
 
   // --------------------------------------------------------- a tile of codes
-  __device__ void tile8(const uint8_t* kc, const uint8_t* vc, const float* ksc, const float* vsc, int tile, int main_len) {
-    const int t0 = tile * TILE, r = n;
-    u4 kr[4][NC > 0 ? NC : 1];
-    u2 kx[4];
+  // In registers as loaded. The next tile's keys are loaded when the scores have
+  // taken this one's, its values when the output has, so that a wave always has
+  // half a tile on the way.
+  u4 kr[4][NC];
+  u2 kx[4];
+  u4 vr[NO];
+  float ks, vs;
+
+  __device__ void load_k(const uint8_t* kc, const float* ksc, int tile) {
+    // a uniform base per tile, one lane offset for all of them
+    const uint8_t* kp = kc + (int64_t)tile * (TILE * D);
+    const uint32_t row = (16 * (n >> 2) + (n & 3)) * D, at = row + g * 16, ax = row + NC * 64 + g * 8;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      const uint8_t* kp = kc + (int64_t)(t0 + 16 * (r >> 2) + 4 * s + (r & 3)) * D;
 #pragma unroll
-      for (int c = 0; c < NC; ++c) kr[s][c] = *(const u4*)(kp + c * 64 + g * 16);
-      if constexpr (ODD) kx[s] = *(const u2*)(kp + NC * 64 + g * 8);
+      for (int c = 0; c < NC; ++c) kr[s][c] = *(const u4*)(kp + (at + s * 4 * D + c * 64));
+      if constexpr (ODD) kx[s] = *(const u2*)(kp + (ax + s * 4 * D));
     }
-    const int blk = (t0 + 16 * g) >> p.block_shift;
-    const float ks = ksc[blk], vs = vsc[blk];
-    u4 vr[NO];
-    const uint8_t* vp = vc + ((int64_t)tile * D + r) * TILE + g * 16;
+    ks = ksc[(tile * TILE + 16 * g) >> p.block_shift];
+  }
+  __device__ void load_v(const uint8_t* vc, const float* vsc, int tile) {
+    const uint8_t* vp = vc + (int64_t)tile * (D * TILE);
+    const uint32_t at = NO * n * TILE + g * 16;
 #pragma unroll
-    for (int i = 0; i < NO; ++i) vr[i] = *(const u4*)(vp + i * 16 * TILE);
+    for (int i = 0; i < NO; ++i) vr[i] = *(const u4*)(vp + (at + i * TILE));
+    vs = vsc[(tile * TILE + 16 * g) >> p.block_shift];
+  }
 
+  // The tile in registers; `next` (< 0: none) is loaded behind it.
+  __device__ void tile8(const uint8_t* kc, const uint8_t* vc, const float* ksc, const float* vsc, int tile, int next, int main_len) {
+    const int t0 = tile * TILE;
+    if (!AHEAD) load_k(kc, ksc, tile);
     float s[16], w[16];
     const float cs = cn * ks;
 #pragma unroll
@@ -171,20 +183,24 @@ struct Decode {
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[4 * t + i] = acc[i] * cs;
+      if (!AHEAD) __builtin_amdgcn_sched_barrier(0);  // no conversions ahead: registers
     }
-    const bool masked = !whole(t0, main_len);
+    if (AHEAD && next >= 0) load_k(kc, ksc, next);
+    if (!AHEAD) {
+      __builtin_amdgcn_sched_barrier(0);  // the values' registers are the keys'
+      load_v(vc, vsc, tile);
+    }
+    const bool masked = !whole(t0, TILE, main_len);
     if (masked) {
+      const uint32_t seen = seen_bits(t0 + 16 * g, 16, main_len, pos, low, p.sinks);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int t = t0 + 16 * g + i;
-        s[i] = t < main_len && sees(t, pos, low) ? s[i] : -INFINITY;
-      }
+      for (int i = 0; i < 16; ++i) s[i] = seen >> i & 1 ? s[i] : -INFINITY;
       if (t0 + 16 * g >= main_len) {  // not written yet: any bytes
 #pragma unroll
         for (int i = 0; i < NO; ++i) vr[i] = u4{0, 0, 0, 0};
       }
     }
-    weights<true>(s, __builtin_amdgcn_logf(vs), masked, w);
+    weights<true, 16>(s, __builtin_amdgcn_logf(vs), masked, w);
     u4 pw[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -196,143 +212,122 @@ struct Decode {
       o[i] = mma16<false>(u4{a.x, a.y, b.x, b.y}, pw[0], o[i]);
       const u2 e = codes4<FMT, false>(vr[i].z), f = codes4<FMT, false>(vr[i].w);
       o[i] = mma16<false>(u4{e.x, e.y, f.x, f.y}, pw[1], o[i]);
+      if (!AHEAD && i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
+    if (AHEAD && next >= 0) load_v(vc, vsc, next);
+  }
+
+  // ------------------------------------------- half a tile of 16-bit tokens
+  // 32 tokens: row 4a + i of the s-th product is token 8a + 4s + i, and a lane
+  // has the scores of tokens 8g .. 8g + 7, one k-step of the output. Of nv
+  // tokens at rows 0 .. of kb, vb; rows past nv repeat the last one, which no
+  // query sees there. The next half is loaded as the next tile is in tile8.
+  u4 k16[2][NS];
+  uint32_t v16[8][NO / 2];  // dims NO n .. NO n + NO - 1 of 8 tokens
+
+  __device__ void load_k16(const uint16_t* kb, int64_t kst, int nv) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const uint16_t* kp = kb + (int64_t)min(8 * (n >> 2) + 4 * s + (n & 3), nv - 1) * kst;
+#pragma unroll
+      for (int st = 0; st < NS; ++st) k16[s][st] = *(const u4*)(kp + kdim(st, g));
+    }
+  }
+  __device__ void load_v16(const uint16_t* vb, int64_t vst, int nv) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const uint16_t* vp = vb + (int64_t)min(8 * g + u, nv - 1) * vst + NO * n;
+      if constexpr (NO % 8 == 0) {
+#pragma unroll
+        for (int i = 0; i < NO / 8; ++i) {
+          const u4 x = *(const u4*)(vp + 8 * i);
+          v16[u][4 * i] = x.x, v16[u][4 * i + 1] = x.y, v16[u][4 * i + 2] = x.z, v16[u][4 * i + 3] = x.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NO / 2; ++i) v16[u][i] = *(const uint32_t*)(vp + 2 * i);
+      }
     }
   }
 
-  // ------------------------------------------------- a tile of 16-bit tokens
-  // Tokens t0 .. t0 + nv - 1 (1 <= nv <= 64) at rows 0 .. of kb, vb. Rows past
-  // nv repeat the last one; no query sees them.
-  __device__ void tile16(const u4 (&qf)[NS], float c, const uint16_t* kb, int64_t kst, const uint16_t* vb, int64_t vst,
-                         int t0, int nv) {
-    const int r = n;
-    float s[16], w[16];
+  // Tokens t0 .. t0 + nv - 1 (nv <= 32 of them count) in registers; nn > 0: the
+  // next half, of nn tokens at kn, vn, is loaded behind it.
+  __device__ void half16(const u4 (&qf)[NS], float c, int t0, int nv, const uint16_t* kn, int64_t kst, const uint16_t* vn,
+                         int64_t vst, int nn) {
+    if (!AHEAD) load_k16(kn, kst, nv);
+    float s[8], w[8];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const uint16_t* kp = kb + (int64_t)min(16 * (r >> 2) + 4 * t + (r & 3), nv - 1) * kst;
-      u4 kr[NS];
-#pragma unroll
-      for (int st = 0; st < NS; ++st) kr[st] = *(const u4*)(kp + kdim(st, g));
+    for (int t = 0; t < 2; ++t) {
       f4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int st = 0; st < NS; ++st) acc = mma16<BF>(kr[st], qf[st], acc);
+      for (int st = 0; st < NS; ++st) acc = mma16<BF>(k16[t][st], qf[st], acc);
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[4 * t + i] = acc[i] * c;
     }
-    const bool masked = nv < TILE || !whole(t0, t0 + nv);
+    if (AHEAD && nn > 0) load_k16(kn, kst, nn);
+    if (!AHEAD) {
+      __builtin_amdgcn_sched_barrier(0);
+      load_v16(vn, vst, nv);
+    }
+    const bool masked = !whole(t0, HALF, t0 + nv);
+    uint32_t seen = 0xff;
+    if (masked) {
+      seen = seen_bits(t0 + 8 * g, 8, t0 + nv, pos, low, p.sinks);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] = seen >> i & 1 ? s[i] : -INFINITY;
+    }
+    weights<CACHED, 8>(s, 0.f, masked, w);
+    u4 pw, px;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      pw[i] = bits2<BF>(w[2 * i], w[2 * i + 1]);
+      if constexpr (BF) px[i] = bits2<true>(w[2 * i] - elem<true>(pw[i] & 0xffff), w[2 * i + 1] - elem<true>(pw[i] >> 16));
+    }
+    uint32_t odd = 0;
     if (masked) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int t = 16 * g + i;
-        s[i] = t < nv && sees(t0 + t, pos, low) ? s[i] : -INFINITY;
-      }
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int i = 0; i < NO / 2; ++i) odd |= odd16<BF>(v16[u][i]);
     }
-    weights<CACHED>(s, 0.f, masked, w);
+    const bool apart = __any(odd & ODD_BITS);
+    const u4 ones = {seen2<BF>(seen), seen2<BF>(seen >> 2), seen2<BF>(seen >> 4), seen2<BF>(seen >> 6)};
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      u4 pw, px;
+    for (int i = 0; i < NO; ++i) {
+      u4 vf;  // 8 tokens of dim NO n + i
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float a = w[8 * t + 2 * i], b = w[8 * t + 2 * i + 1];
-        pw[i] = bits2<BF>(a, b);
-        if constexpr (BF) px[i] = bits2<true>(a - elem<true>(pw[i] & 0xffff), b - elem<true>(pw[i] >> 16));
+      for (int u = 0; u < 4; ++u)
+        vf[u] = __builtin_amdgcn_perm(v16[2 * u + 1][i / 2], v16[2 * u][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+      if (apart) {
+        const f4 m = mma16<BF>(marks<BF>(vf), ones, f4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[i][k] += marked(m[k]);
       }
-      u4 vf[NO];  // 8 tokens of one dim each
-      if constexpr (CACHED) {
-        // the output's dims as tile8 has them: dim 16 i + r
-#pragma unroll
-        for (int i = 0; i < NO; ++i)
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const uint16_t* v0 = vb + (int64_t)min(16 * g + 8 * t + 2 * u, nv - 1) * vst + i * 16 + r;
-            const uint16_t* v1 = vb + (int64_t)min(16 * g + 8 * t + 2 * u + 1, nv - 1) * vst + i * 16 + r;
-            vf[i][u] = (uint32_t)*v0 | (uint32_t)*v1 << 16;
-          }
-      } else {
-        // dims NO r .. NO r + NO - 1 of 8 tokens, paired by tokens: dim NO r + i
-        uint32_t vr[8][NO / 2];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const uint16_t* vp = vb + (int64_t)min(16 * g + 8 * t + u, nv - 1) * vst + NO * r;
-          if constexpr (NO % 8 == 0) {
-#pragma unroll
-            for (int i = 0; i < NO / 8; ++i) {
-              const u4 x = *(const u4*)(vp + 8 * i);
-              vr[u][4 * i] = x.x, vr[u][4 * i + 1] = x.y, vr[u][4 * i + 2] = x.z, vr[u][4 * i + 3] = x.w;
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < NO / 2; ++i) vr[u][i] = *(const uint32_t*)(vp + 2 * i);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < NO; ++i)
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            vf[i][u] = __builtin_amdgcn_perm(vr[2 * u + 1][i / 2], vr[2 * u][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
-      }
-      bool odd = false;
-      if (masked) {  // an infinite or NaN value among the tile's?
-        const uint32_t ex = BF ? 0x7f80u : 0x7c00u;
-#pragma unroll
-        for (int i = 0; i < NO; ++i)
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            odd |= (vf[i][u] & ex) == ex || (vf[i][u] & ex << 16) == ex << 16;
-      }
-      if (__any(odd)) {
-#pragma unroll
-        for (int i = 0; i < NO; ++i) {
-#pragma unroll 1
-          for (int row = 0; row < DEC_ROWS; ++row) {
-            const int at = __shfl(pos, row), lw = __shfl(low, row);
-            u4 v = vf[i];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int k = 16 * g + 8 * t + 2 * u;
-              v[u] &= (k < nv && sees(t0 + k, at, lw) ? 0xffffu : 0u) | (k + 1 < nv && sees(t0 + k + 1, at, lw) ? 0xffff0000u : 0u);
-            }
-            f4 x = mma16<BF>(v, pw, f4{0.f, 0.f, 0.f, 0.f});
-            if constexpr (BF) x = mma16<BF>(finite(v), px, x);
-            o[i] = n == row ? o[i] + x : o[i];
-          }
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < NO; ++i) {
-          o[i] = mma16<BF>(vf[i], pw, o[i]);
-          if constexpr (BF) o[i] = mma16<BF>(vf[i], px, o[i]);
-        }
-      }
+      o[i] = mma16<BF>(vf, pw, o[i]);
+      if constexpr (BF) o[i] = mma16<BF>(vf, px, o[i]);
+      if (!AHEAD && i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
-  }
-  // infinite and NaN values as 0: the weights' remainders may be 0
-  static __device__ u4 finite(u4 v) {
-    const uint32_t ex = BF ? 0x7f80u : 0x7c00u;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if ((v[u] & ex) == ex) v[u] &= 0xffff0000u;
-      if ((v[u] & ex << 16) == ex << 16) v[u] &= 0xffffu;
-    }
-    return v;
+    if (AHEAD && nn > 0) load_v16(vn, vst, nn);
   }
 };
 
+// One (sequence, kv head): places first .. last - 1 of its list (those past its
+// tiles hold none), to the output (slot < 0) or to partial slot `slot`.
 template <int D, bool BF, int FMT>
-__global__ __launch_bounds__(DEC_WAVES * 64) void decode_kernel(const Params p) {
-  constexpr bool CACHED = FMT != DENSE;
+__device__ inline void decode_unit(const Params& p, int b, int h, int first, int last, int slot) {
+  constexpr bool CACHED = FMT != DENSE, AHEAD = Decode<D, BF, FMT>::AHEAD;
   constexpr int PASS = D > 128 ? 2 : 1;      // of the output through LDS
   constexpr int NO = D / 16, NP = NO / PASS;
   __shared__ float os[DEC_WAVES][DEC_ROWS][NP * 16 + 4];
   __shared__ float ml[DEC_WAVES][DEC_ROWS][4];
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int split = blockIdx.x % p.splits, bh = blockIdx.x / p.splits;
-  const int b = bh / p.hkv, h = bh - b * p.hkv;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int bh = b * p.hkv + h;
   const int len = length_of(p, b);
   const int pmin = len - p.n_q, pmax = len - 1;
   const Tiles tl = tiles_of(len, CACHED, p.block_shift, pmin, pmax, p.window, p.sinks);
-  const int first = split * p.chunk, last = min(tl.n, first + p.chunk);
-  if (p.splits > 1 && first >= tl.n) return;  // the merge kernel counts the same tiles
+
+  last = min(last, tl.n);
 
   Decode<D, BF, FMT> w(p);
   w.n = lane & 15;
@@ -346,12 +341,10 @@ __global__ __launch_bounds__(DEC_WAVES * 64) void decode_kernel(const Params p) 
   w.lowmax = p.window ? pmax - p.window : -1;
   w.M = w.m = -INFINITY;
   w.l = 0.f;
+#pragma unroll
   for (int i = 0; i < NO; ++i) w.o[i] = f4{0.f, 0.f, 0.f, 0.f};
-
   const uint16_t* qp = (const uint16_t*)p.q.p + (int64_t)b * p.q.sb + (int64_t)(h * p.group + head) * p.q.sh + (int64_t)qi * p.q.st;
-  w.load_q(qp, live, w.q);
   w.cn = p.scale;
-  if constexpr (CACHED && BF) w.cn *= w.to_f16(w.q);
 
   if constexpr (CACHED) {
     const int64_t row = bh;
@@ -359,29 +352,61 @@ __global__ __launch_bounds__(DEC_WAVES * 64) void decode_kernel(const Params p) 
     const uint8_t* vc = p.v_codes + row * p.cap * D;
     const float* ksc = p.k_scales + row * (p.cap >> p.block_shift);
     const float* vsc = p.v_scales + row * (p.cap >> p.block_shift);
-    for (int i = first + wave; i < last; i += DEC_WAVES) {
-      if (i < tl.n_main) {
-        w.tile8(kc, vc, ksc, vsc, tl.at(i), tl.main_len);
-      } else {
-        u4 qt[D / 32];
-        w.load_q(qp, live, qt);
-        w.tile16(qt, p.scale, p.k_tail + (row << p.block_shift) * D, D, p.v_tail + (row << p.block_shift) * D, D,
-                 tl.main_len, len - tl.main_len);
+    const int end = min(last, tl.n_main);
+    int i = first + wave;
+    if (AHEAD && i < end) {
+      w.load_k(kc, ksc, tl.at(i));
+      w.load_v(vc, vsc, tl.at(i));
+    }
+    w.load_q(qp, live, w.q);
+    if constexpr (BF) w.cn *= w.to_f16(w.q);
+    for (; i < end; i += DEC_WAVES)
+      w.tile8(kc, vc, ksc, vsc, tl.at(i), i + DEC_WAVES < end ? tl.at(i + DEC_WAVES) : -1, tl.main_len);
+    if (i < last) {  // the tail
+      u4 qt[D / 32];
+      w.load_q(qp, live, qt);
+      const uint16_t *kt = p.k_tail + (row << p.block_shift) * D, *vt = p.v_tail + (row << p.block_shift) * D;
+      const int nt = len - tl.main_len;
+      if constexpr (AHEAD) {
+        w.load_k16(kt, D, nt);
+        w.load_v16(vt, D, nt);
+      }
+      for (int t = 0; t < nt; t += HALF) {
+        const int at = AHEAD ? t + HALF : t;
+        w.half16(qt, p.scale, tl.main_len + t, min(nt - t, HALF), kt + at * D, D, vt + at * D, D, nt - t - HALF);
       }
     }
   } else {
+    w.load_q(qp, live, w.q);
     const uint16_t* kb = (const uint16_t*)p.k.p + (int64_t)b * p.k.sb + (int64_t)h * p.k.sh;
     const uint16_t* vb = (const uint16_t*)p.v.p + (int64_t)b * p.v.sb + (int64_t)h * p.v.sh;
-    for (int i = first + wave; i < last; i += DEC_WAVES) {
-      const int t0 = tl.at(i) * TILE;
-      w.tile16(w.q, p.scale, kb + (int64_t)t0 * p.k.st, p.k.st, vb + (int64_t)t0 * p.v.st, p.v.st, t0, min(TILE, len - t0));
+    // halves of the wave's tiles, in order: the tokens from `t0` on
+    int i = first + wave;
+    if (i < last) {
+      int t0 = tl.at(i) * TILE;
+      if constexpr (AHEAD) {
+        w.load_k16(kb + (int64_t)t0 * p.k.st, p.k.st, len - t0);
+        w.load_v16(vb + (int64_t)t0 * p.v.st, p.v.st, len - t0);
+      }
+      for (;;) {
+        int next = t0 + HALF;
+        if (!(t0 & HALF) && next < len) {
+          // the tile's other half
+        } else {
+          i += DEC_WAVES;
+          next = i < last ? tl.at(i) * TILE : len;
+        }
+        const int64_t at = AHEAD ? next : t0;
+        w.half16(w.q, p.scale, t0, min(HALF, len - t0), kb + at * p.k.st, p.k.st, vb + at * p.v.st, p.v.st, len - next);
+        if (next >= len) break;
+        t0 = next;
+      }
     }
   }
 
   // the row's sum over its four lanes
   if constexpr (CACHED) {
-    float mt = fmaxf(w.m, __shfl_xor(w.m, 16));
-    mt = fmaxf(mt, __shfl_xor(mt, 32));
+    const float mt = lanes_max<16>(w.m);
     w.l *= __builtin_amdgcn_exp2f(w.m - (mt == -INFINITY ? 0.f : mt));
     w.m = mt;
   } else {
@@ -410,8 +435,8 @@ __global__ __launch_bounds__(DEC_WAVES * 64) void decode_kernel(const Params p) 
         f[v] = __builtin_amdgcn_exp2f(ml[v][orow][0] - Mr);
         l += ml[v][orow][2] * __builtin_amdgcn_exp2f(ml[v][orow][1] - mr);
       }
-      if (p.splits > 1 && orow < p.rows && (threadIdx.x & 15) == 0) {
-        float* d = p.ws + (((int64_t)bh * p.rows + orow) * p.splits + split) * 4;
+      if (slot >= 0 && orow < p.rows && (threadIdx.x & 15) == 0) {
+        float* d = p.ws + ((int64_t)slot * p.rows + orow) * 4;
         d[0] = M, d[1] = m, d[2] = l;
       }
     }
@@ -419,14 +444,12 @@ __global__ __launch_bounds__(DEC_WAVES * 64) void decode_kernel(const Params p) 
     const float Mr = M == -INFINITY ? 0.f : M, mr = m == -INFINITY ? 0.f : m;
     const float fin = CACHED ? __builtin_amdgcn_exp2f(Mr - mr) : 1.f;
     for (int k = threadIdx.x & 15; k < NP * 16; k += 16) {
-      // column k in the order of the output's dims
-      const int i = CACHED ? k >> 4 : k % NP, r = CACHED ? k & 15 : k / NP;
-      const int dim = CACHED ? (ps * NP + i) * 16 + r : NO * r + ps * NP + i;
+      const int i = k % NP, r = k / NP, dim = NO * r + ps * NP + i;  // in the order of the dims
       float x = 0.f;
 #pragma unroll
       for (int v = 0; v < DEC_WAVES; ++v) x += os[v][orow][i * 16 + r] * f[v];
-      if (p.splits > 1) {
-        p.ws[p.o_off + (((int64_t)bh * p.rows + orow) * p.splits + split) * D + dim] = x;
+      if (slot >= 0) {
+        p.ws[p.o_off + ((int64_t)slot * p.rows + orow) * D + dim] = x;
       } else {
         x = pmin + oi < 0 ? 0.f : x / l * fin;
         const int64_t at = (int64_t)b * p.out.sb + (int64_t)(h * p.group + oh) * p.out.sh + (int64_t)oi * p.out.st + dim;
@@ -440,8 +463,42 @@ __global__ __launch_bounds__(DEC_WAVES * 64) void decode_kernel(const Params p) 
 }
 
 template <int D, bool BF, int FMT>
+__global__ __launch_bounds__(DEC_WAVES * 64, 2) void decode_kernel(const Params p) {
+  constexpr bool CACHED = FMT != DENSE;
+  int b, h, n, i = 0;      // sequence, kv head, its places, the first one to do
+  int at = 0, end;         // of the list
+  if (p.wgs == 0) {
+    b = blockIdx.x / p.hkv;
+    h = blockIdx.x - b * p.hkv;
+    end = n = decode_places(p, CACHED, b);
+  } else {
+    int before;
+    const Share s = share_of(p, CACHED, blockIdx.x, b, before);
+    if (b < 0) return;
+    at = blockIdx.x * s.per;
+    end = min(s.total, at + s.per);
+    n = decode_places(p, CACHED, b);
+    h = (at - before) / n;
+    i = at - before - h * n;
+  }
+  for (;;) {
+    const int last = min(n, i + end - at);
+    decode_unit<D, BF, FMT>(p, b, h, i, last, p.wgs == 0 ? -1 : blockIdx.x + b * p.hkv + h);
+    at += last - i;
+    if (at >= end) return;
+    i = 0;
+    if (++h == p.hkv) {
+      h = 0;
+      do n = decode_places(p, CACHED, ++b);
+      while (n == 0);  // ends: the list has places left
+    }
+    __syncthreads();  // the last unit's reads of LDS
+  }
+}
+
+template <int D, bool BF, int FMT>
 hipError_t launch_decode_as(const Params& p, hipStream_t stream) {
-  decode_kernel<D, BF, FMT><<<(uint32_t)(p.splits * p.batch * p.hkv), DEC_WAVES * 64, 0, stream>>>(p);
+  decode_kernel<D, BF, FMT><<<(uint32_t)(p.wgs ? p.wgs : p.batch * p.hkv), DEC_WAVES * 64, 0, stream>>>(p);
   return hipGetLastError();
 }
 

@@ -91,9 +91,8 @@ class KVAttnDesc(ctypes.Structure):
                 ("len_b", _p), ("scale", ctypes.c_float), ("q", Rows4), ("out", Rows4), ("k", Rows4), ("v", Rows4)]
 
 
-_P8 = ctypes.POINTER(KV8StoreDesc)
-_PR = ctypes.POINTER(Rows4)
-_PK = ctypes.POINTER(KVAttnDesc)
+# void pointers: the callers pass these three packed as bytes
+_P8 = _PR = _PK = _p
 _PC = ctypes.POINTER(Codec)
 _PS = ctypes.POINTER(Store)
 _PSp = ctypes.POINTER(Span)

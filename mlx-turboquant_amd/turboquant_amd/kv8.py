@@ -31,7 +31,7 @@ by inference.
 from __future__ import annotations
 
 import contextlib
-import ctypes
+import struct
 
 import numpy as np
 import torch
@@ -44,25 +44,43 @@ BLOCKS = (16, 32, 64)
 FORMATS = {"int8": (_lib.TQ_KV8_INT8, torch.int8), "fp8": (_lib.TQ_KV8_E4M3, torch.float8_e4m3fn)}
 
 
+# The C structs as bytes: packing them takes a fraction of the time that filling
+# ctypes structures does, which a decode step's host path would wait for.
+_STORE = struct.Struct("@6Pq6i")
+_ROWS = struct.Struct("@Pqqq")
+_DESC = struct.Struct("@10iPf4x" + "Pqqq" * 4)
+_NO_ROWS = (0, 0, 0, 0)
+
+_NULL = contextlib.nullcontext()
+_current_device = torch.cuda.current_device
+
+
 def _on(device: torch.device):
     """Launches go to the tensors' own device, whichever is current."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    return _NULL if device.index is None or device.index == _current_device() else torch.cuda.device(device)
 
 
-def _rows4(t: torch.Tensor) -> tuple[_lib.Rows4, torch.Tensor]:
-    """``tq_rows4`` of (B, H, T, D), and the tensor it points into (a copy
-    where the kernels cannot take its strides or address)."""
-    sb, sh, st = (0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3]))
-    if t.stride(3) != 1 or (sb | sh | st) % 8 or t.data_ptr() % 16:
-        t = t.contiguous().clone() if t.data_ptr() % 16 else t.contiguous()
-        sb, sh, st = t.stride()[:3]
-    return _lib.Rows4(t.data_ptr(), sb, sh, st), t
+def _rows4(t: torch.Tensor) -> tuple[tuple[int, int, int, int], torch.Tensor]:
+    """The fields of a ``tq_rows4`` of (B, H, T, D), and the tensor it points
+    into (a copy where the kernels cannot take its strides or address)."""
+    nb, nh, nt, _ = t.shape
+    sb, sh, st, sd = t.stride()
+    p = t.data_ptr()
+    if nb == 1:
+        sb = 0
+    if nh == 1:
+        sh = 0
+    if nt == 1:
+        st = 0
+    if sd != 1 or (sb | sh | st) & 7 or p & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        sb, sh, st, _ = t.stride()
+        p = t.data_ptr()
+    return (p, sb, sh, st), t
 
 
-def _lengths(lens, batch: int, cap: int, device, what: str) -> tuple[int | None, int]:
-    """(device array or None, the length where there is one for all)."""
+def _lengths(lens, batch: int, cap: int, device, what: str) -> tuple[int, int]:
+    """(device array or 0, the length where there is one for all)."""
     if isinstance(lens, torch.Tensor):
         if lens.dtype != torch.int32 or lens.shape != (batch,) or lens.device != device or not lens.is_contiguous():
             raise ValueError(f"{what}: an int, or a contiguous int32 tensor of shape ({batch},) on {device}")
@@ -70,7 +88,7 @@ def _lengths(lens, batch: int, cap: int, device, what: str) -> tuple[int | None,
     n = int(lens)
     if not 0 <= n <= cap:
         raise ValueError(f"{what} {n} outside [0, {cap}]")
-    return None, n
+    return 0, n
 
 
 class KV8Store:
@@ -107,26 +125,23 @@ class KV8Store:
     def _set(self, fmt, k_codes, v_codes, k_scales, v_scales, k_tail, v_tail) -> None:
         B, H, cap, D = k_codes.shape
         block = k_tail.shape[2]
-        code = FORMATS[fmt][1]
+        code, dev, dtype = FORMATS[fmt][1], k_codes.device, k_tail.dtype
         if cap % TILE:
             raise ValueError(f"k_codes: room for {cap} tokens, not a multiple of {TILE}")
-        for name, t, shape, dtype in (("k_codes", k_codes, (B, H, cap, D), code),
-                                      ("v_codes", v_codes, (B, H, cap // TILE, D, TILE), code),
-                                      ("k_scales", k_scales, (B, H, cap // block), torch.float32),
-                                      ("v_scales", v_scales, (B, H, cap // block), torch.float32),
-                                      ("k_tail", k_tail, (B, H, block, D), k_tail.dtype),
-                                      ("v_tail", v_tail, (B, H, block, D), k_tail.dtype)):
-            if t.shape != shape or t.dtype != dtype or not t.is_contiguous() or t.device != k_codes.device:
-                raise ValueError(f"{name}: expected a contiguous {dtype} tensor of shape {shape} on {k_codes.device}, got "
+        scales, tail = (B, H, cap // block), (B, H, block, D)
+        for t, shape, kind in ((k_codes, k_codes.shape, code), (v_codes, (B, H, cap // TILE, D, TILE), code),
+                               (k_scales, scales, torch.float32), (v_scales, scales, torch.float32),
+                               (k_tail, tail, dtype), (v_tail, tail, dtype)):
+            if t.shape != shape or t.dtype != kind or t.device != dev or not t.is_contiguous():
+                raise ValueError(f"store: expected a contiguous {kind} tensor of shape {tuple(shape)} on {dev}, got "
                                  f"{t.dtype} {tuple(t.shape)} on {t.device}")
         self.fmt, self.block, self.batch, self.heads, self.cap, self.head_dim = fmt, block, B, H, cap, D
-        self.dtype, self.device = k_tail.dtype, k_codes.device
+        self.dtype, self.device = dtype, dev
         self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
         self.k_tail, self.v_tail = k_tail, v_tail
-        self.desc = _lib.KV8StoreDesc(
-            k_codes=k_codes.data_ptr(), v_codes=v_codes.data_ptr(), k_scales=k_scales.data_ptr(),
-            v_scales=v_scales.data_ptr(), k_tail=k_tail.data_ptr(), v_tail=v_tail.data_ptr(), cap=cap,
-            fmt=FORMATS[fmt][0], d=D, block=block, kv_dtype=_lib.dtype_code(self.dtype), batch=B, heads=H)
+        self.desc = _STORE.pack(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+                                k_tail.data_ptr(), v_tail.data_ptr(), cap, FORMATS[fmt][0], D, block, _lib.dtype_code(dtype),
+                                B, H)
 
     def tensors(self) -> dict:
         """The arrays by the names that ``from_tensors`` takes."""
@@ -164,10 +179,16 @@ def _check(fmt: str, head_dim: int, block: int, dtype) -> None:
         raise ValueError(f"keys and values of {dtype} not supported: fp16 or bf16")
 
 
-def _ready(store: KV8Store) -> None:
-    if store.device.type != "cuda":
-        raise RuntimeError("turboquant_amd runs on the GPU only; got a CPU tensor")
-    _codec._require_gfx950(store.device)
+_devices: set[torch.device] = set()
+
+
+def _ready(device: torch.device) -> None:
+    """Refuse what is not a gfx950 device (looked up once per device)."""
+    if device not in _devices:
+        if device.type != "cuda":
+            raise RuntimeError("turboquant_amd runs on the GPU only; got a CPU tensor")
+        _codec._require_gfx950(device)
+        _devices.add(device)
 
 
 def kv8_write(store: KV8Store, keys: torch.Tensor, values: torch.Tensor, start, n_new: torch.Tensor | None = None) -> None:
@@ -181,25 +202,25 @@ def kv8_write(store: KV8Store, keys: torch.Tensor, values: torch.Tensor, start, 
     the host: a sequence whose tokens would not fit, or whose start or count is
     negative (or n_new > T), is left as it is."""
     B, H, D = store.batch, store.heads, store.head_dim
+    T = keys.shape[2] if keys.dim() == 4 else 0
     for name, t in (("keys", keys), ("values", values)):
-        if t.dim() != 4 or t.shape[0] != B or t.shape[1] != H or t.shape[3] != D or t.shape != keys.shape:
-            raise ValueError(f"{name}: expected ({B}, {H}, T, {D}) like the store, got {tuple(t.shape)}")
+        if t.shape != (B, H, T, D):
+            raise ValueError(f"{name}: expected ({B}, {H}, T, {D}) like the store, one T for both, got {tuple(t.shape)}")
         if t.dtype != store.dtype or t.device != store.device:
             raise ValueError(f"{name}: expected {store.dtype} on {store.device}, got {t.dtype} on {t.device}")
-    T = keys.shape[2]
     if T > store.cap:
         raise ValueError(f"{T} tokens > the {store.cap} there is room for")
     start_b, s0 = _lengths(start, B, store.cap - T, store.device, "start")
-    count_b = _lengths(n_new, B, T, store.device, "n_new")[0] if isinstance(n_new, torch.Tensor) else None
-    if n_new is not None and count_b is None:
+    if n_new is not None and not isinstance(n_new, torch.Tensor):
         raise ValueError("n_new: None, or an int32 tensor of one count per sequence")
+    count_b = 0 if n_new is None else _lengths(n_new, B, T, store.device, "n_new")[0]
     if T == 0 or B == 0:
         return
-    _ready(store)
+    _ready(store.device)
     (k, keys), (v, values) = _rows4(keys), _rows4(values)
     lib = _lib.load()
     with _on(store.device):
-        _lib.check(lib.tq_kv8_write(ctypes.byref(store.desc), ctypes.byref(k), ctypes.byref(v), start_b, s0, count_b, T,
+        _lib.check(lib.tq_kv8_write(store.desc, _ROWS.pack(*k), _ROWS.pack(*v), start_b, s0, count_b, T,
                                     _lib.stream_ptr(store.device)), "tq_kv8_write")
 
 
@@ -215,7 +236,7 @@ def kv8_read(store: KV8Store, lens, start: int = 0, n: int | None = None,
     B, H, D = store.batch, store.heads, store.head_dim
     len_b, length = _lengths(lens, B, store.cap, store.device, "lens")
     if n is None:
-        n = max(0, (store.cap if len_b is not None else length) - start)
+        n = max(0, (store.cap if len_b else length) - start)
     if start < 0 or n < 0 or start + n > store.cap:
         raise ValueError(f"tokens {start} .. {start + n - 1} outside the store's {store.cap}")
     dtype = store.dtype if dtype is None else dtype
@@ -224,18 +245,19 @@ def kv8_read(store: KV8Store, lens, start: int = 0, n: int | None = None,
     v = torch.empty_like(k)
     if n == 0 or B == 0:
         return k, v
-    _ready(store)
+    _ready(store.device)
     lib = _lib.load()
     with _on(store.device):
-        _lib.check(lib.tq_kv8_read(ctypes.byref(store.desc), len_b, length, start, n, code, k.data_ptr(), v.data_ptr(),
+        _lib.check(lib.tq_kv8_read(store.desc, len_b, length, start, n, code, k.data_ptr(), v.data_ptr(),
                                    _lib.stream_ptr(store.device)), "tq_kv8_read")
     return k, v
 
 
-def _attention_desc(queries, B, hkv, D, dtype, device, len_b, max_len, scale, window, sinks, out):
-    """(descriptor, output, tensors to keep until the launch) of an attention call."""
-    q = queries if queries.dim() == 4 else queries[:, :, None] if queries.dim() == 3 else None
-    if q is None or q.shape[0] != B or q.shape[3] != D or q.shape[1] % hkv or q.shape[1] == 0:
+def _attention_desc(queries, B, hkv, D, dtype, device, len_b, max_len, scale, window, sinks, out, k=_NO_ROWS, v=_NO_ROWS):
+    """(``tq_kv_attn_desc`` as bytes, output, tensor to keep until the launch) of an attention call."""
+    q = queries[:, :, None] if queries.dim() == 3 else queries
+    shape = q.shape
+    if len(shape) != 4 or shape[0] != B or shape[3] != D or shape[1] % hkv or shape[1] == 0:
         raise ValueError(f"query shape {tuple(queries.shape)} does not match {B} sequences of {hkv} kv heads, head_dim {D}")
     if q.dtype != dtype or q.device != device:
         raise ValueError(f"queries: expected {dtype} on {device}, got {q.dtype} on {q.device}")
@@ -243,20 +265,24 @@ def _attention_desc(queries, B, hkv, D, dtype, device, len_b, max_len, scale, wi
         raise ValueError(f"window {window}: at least 1, or None")
     if sinks < 0:
         raise ValueError(f"sinks {sinks}")
+    code = out_code = _lib.dtype_code(dtype)
     if out is None:
-        out = torch.empty(q.shape, dtype=dtype, device=device)
-    elif out.shape != q.shape or out.dtype not in (dtype, torch.float32) or out.device != device:
-        raise ValueError(f"out: expected {tuple(q.shape)} of {dtype} or float32 on {device}")
-    o, same = _rows4(out)
-    if same is not out:
-        raise ValueError("out: rows must be contiguous and 16-byte aligned, strides multiples of 8")
+        out = torch.empty(shape, dtype=dtype, device=device)
+        o = (out.data_ptr(), *out.stride()[:3])
+    else:
+        if out.shape != shape or out.dtype not in (dtype, torch.float32) or out.device != device:
+            raise ValueError(f"out: expected {tuple(shape)} of {dtype} or float32 on {device}")
+        o, same = _rows4(out)
+        if same is not out:
+            raise ValueError("out: rows must be contiguous and 16-byte aligned, strides multiples of 8")
+        out_code = _lib.dtype_code(out.dtype)
     rows, q = _rows4(q)
-    most = 2 ** 31 - 1
-    desc = _lib.KVAttnDesc(
-        batch=B, hq=q.shape[1], hkv=hkv, d=D, n_q=q.shape[2], dtype=_lib.dtype_code(dtype),
-        out_dtype=_lib.dtype_code(out.dtype), window=0 if window is None else min(window, most), sinks=min(sinks, most),
-        max_len=max_len, len_b=len_b, scale=D ** -0.5 if scale is None else scale, q=rows, out=o)
+    desc = _DESC.pack(B, shape[1], hkv, D, shape[2], code, out_code, 0 if window is None else min(window, _MOST),
+                      min(sinks, _MOST), max_len, len_b, D ** -0.5 if scale is None else scale, *rows, *o, *k, *v)
     return desc, out, q
+
+
+_MOST = 2 ** 31 - 1
 
 
 def kv8_attention(queries: torch.Tensor, store: KV8Store, lens, max_len: int | None = None, scale: float | None = None,
@@ -278,20 +304,20 @@ def kv8_attention(queries: torch.Tensor, store: KV8Store, lens, max_len: int | N
     float32; the softmax's weights are rounded to 16 bits."""
     D, B, H = store.head_dim, store.batch, store.heads
     len_b, length = _lengths(lens, B, store.cap, store.device, "lens")
-    if len_b is not None:
+    if len_b:
         length = store.cap if max_len is None else int(max_len)
         if not 0 <= length <= store.cap:
             raise ValueError(f"max_len {length} outside [0, {store.cap}]")
     desc, out, q = _attention_desc(queries, B, H, D, store.dtype, store.device, len_b, length, scale, window, sinks, out)
     if out.numel() == 0:
         return out
-    _ready(store)
+    _ready(store.device)
     lib = _lib.load()
     with _on(store.device):
-        need = lib.tq_kv8_attention_workspace_bytes(ctypes.byref(store.desc), ctypes.byref(desc))
+        need = lib.tq_kv8_attention_workspace_bytes(store.desc, desc)
         # its own block per call: calls on other streams and captured graphs share nothing
         ws = torch.empty(need, dtype=torch.uint8, device=store.device) if need else None
-        _lib.check(lib.tq_kv8_attention(ctypes.byref(store.desc), ctypes.byref(desc), _lib.ptr(ws), need,
+        _lib.check(lib.tq_kv8_attention(store.desc, desc, _lib.ptr(ws), need,
                                         _lib.stream_ptr(store.device)), "tq_kv8_attention")
     return out
 

@@ -9,12 +9,10 @@ that a query sees are read.
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
-from . import _codec, _lib
-from .kv8 import HEAD_DIMS, _attention_desc, _lengths, _on, _rows4
+from . import _lib
+from .kv8 import _NO_ROWS, HEAD_DIMS, _attention_desc, _lengths, _on, _ready, _rows4
 
 
 def window_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor, window: int | None = None,
@@ -45,19 +43,19 @@ def window_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
     if H == 0:
         raise ValueError("no kv heads")
     len_b, length = _lengths(T if lens is None else lens, B, T, keys.device, "lens")
-    if len_b is not None:
+    if len_b:
         length = T
-    desc, out, q = _attention_desc(queries, B, H, D, keys.dtype, keys.device, len_b, length, scale, window, sinks, out)
+    k = v = _NO_ROWS
+    if length:
+        (k, keys), (v, values) = _rows4(keys), _rows4(values)
+    device = keys.device
+    desc, out, q = _attention_desc(queries, B, H, D, keys.dtype, device, len_b, length, scale, window, sinks, out, k, v)
     if out.numel() == 0:
         return out
-    _lib.require_device(keys)
-    _codec._require_gfx950(keys.device)
-    if length:
-        (desc.k, keys), (desc.v, values) = _rows4(keys), _rows4(values)
+    _ready(device)
     lib = _lib.load()
-    with _on(keys.device):
-        need = lib.tq_window_attention_workspace_bytes(ctypes.byref(desc))
-        ws = torch.empty(need, dtype=torch.uint8, device=keys.device) if need else None
-        _lib.check(lib.tq_window_attention(ctypes.byref(desc), _lib.ptr(ws), need, _lib.stream_ptr(keys.device)),
-                   "tq_window_attention")
+    with _on(device):
+        need = lib.tq_window_attention_workspace_bytes(desc)
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        _lib.check(lib.tq_window_attention(desc, _lib.ptr(ws), need, _lib.stream_ptr(device)), "tq_window_attention")
     return out

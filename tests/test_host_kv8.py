@@ -44,6 +44,23 @@ def test_struct_layouts_match_header():
             assert int(got[f"{cname}.{f}"]) == getattr(cls, f).offset, f"{cname}.{f}"
 
 
+def test_packed_structs_match():
+    """The bytes that the Python layer packs, read as the structs."""
+    from turboquant_amd import kv8
+    s = store(1, 2, 96, 192, "fp8", 16, torch.bfloat16)
+    d = _lib.KV8StoreDesc.from_buffer_copy(s.desc)
+    assert len(s.desc) == ctypes.sizeof(d) and (d.cap, d.fmt, d.d, d.block, d.kv_dtype, d.batch, d.heads) == (192, 1, 96, 16, 1, 1, 2)
+    assert [getattr(d, n) for n in s.tensors()] == [t.data_ptr() for t in s.tensors().values()]
+    q, out = x(1, 4, 3, 96), x(1, 3, 4, 96).float().transpose(1, 2)
+    b, o, _ = kv8._attention_desc(q, 1, 2, 96, H16, q.device, 16, 100, 0.5, 7, 3, out, (32, 1, 2, 3), (48, 4, 5, 6))
+    d = _lib.KVAttnDesc.from_buffer_copy(b)
+    assert len(b) == ctypes.sizeof(d) and o is out
+    assert [getattr(d, n) for n, _ in d._fields_[:12]] == [1, 4, 2, 96, 3, 0, 2, 7, 3, 100, 16, 0.5]
+    assert [[getattr(r, n) for n, _ in r._fields_] for r in (d.q, d.out, d.k, d.v)] == [
+        [q.data_ptr(), 0, 3 * 96, 96], [out.data_ptr(), 0, 96, 4 * 96], [32, 1, 2, 3], [48, 4, 5, 6]]
+    assert bytes(_lib.Rows4(1, 2, 3, 4)) == kv8._ROWS.pack(1, 2, 3, 4)
+
+
 @pytest.mark.parametrize("kw,what", [
     (dict(D=80), "head_dim 80"), (dict(D=512), "head_dim 512"), (dict(block=48), "blocks of 48"), (dict(fmt="int4"), "format"),
     (dict(dtype=torch.float32), "float32"), (dict(cap=-1), "capacity"),
