@@ -25,10 +25,16 @@ constexpr int HALF = TILE / 2;
 constexpr int DEC_WAVES = 4, DEC_ROWS = 16;            // tq_kv_decode.h: waves and most rows per workgroup
 constexpr int CH_WAVES = 4, CH_ROWS = CH_WAVES * 32;   // tq_kv_chunk.h
 constexpr int DENSE = -1;    // format of uncompressed keys and values (else TQ_KV8_*)
-// The reference of the softmax's weights is kept this far (in base 2) below the
-// running maximum: weights up to 2^14 in fp16, which leaves those down to 2^-28
-// of the largest normal, and smaller ones 2^-39 apart.
-constexpr float W_SHIFT = 14.f;
+// The reference of the softmax's weights, in base 2: this far below the running
+// maximum. fp16 weights then reach 2^14, which leaves those down to 2^-28 of the
+// largest normal, and smaller ones 2^-39 apart; bf16 weights stay below 2^-12,
+// so that sums over 2^12 tokens of bf16's largest values stay finite.
+template <bool BF>
+constexpr float W_SHIFT = BF ? -20.f : 13.f;
+// The chunk kernel moves its reference only when a weight would grow past this
+// (in base 2) above what W_SHIFT allows: few tiles do after the first ones.
+template <bool BF>
+constexpr float W_SLACK = BF ? 8.f : 1.f;
 constexpr float QMAX_INT8 = 127.f, QMAX_E4M3 = 448.f;
 constexpr float TINY = 0x1p-110f;  // blocks below are stored as 0: QMAX / a stays finite
 
@@ -43,11 +49,20 @@ __device__ inline u2 int8x4_f16(uint32_t w) {
 }
 
 // Four int8 codes to two dwords of exact bf16 (7 significant bits): the upper
-// halves of their float32 values.
+// halves of their float32 values. One instruction per code, which the compiler
+// makes two of.
+template <int BYTE>
+__device__ inline uint32_t int8_f32(uint32_t w) {
+  uint32_t r;
+  if constexpr (BYTE == 0) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(r) : "v"(w));
+  if constexpr (BYTE == 1) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(r) : "v"(w));
+  if constexpr (BYTE == 2) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(r) : "v"(w));
+  if constexpr (BYTE == 3) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(r) : "v"(w));
+  return r;
+}
 __device__ inline u2 int8x4_bf16(uint32_t w) {
-  const float a = (float)(int8_t)w, b = (float)(int8_t)(w >> 8), c = (float)(int8_t)(w >> 16), d = (float)(int8_t)(w >> 24);
-  return u2{__builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u),
-            __builtin_amdgcn_perm(__float_as_uint(d), __float_as_uint(c), 0x07060302u)};
+  return u2{__builtin_amdgcn_perm(int8_f32<1>(w), int8_f32<0>(w), 0x07060302u),
+            __builtin_amdgcn_perm(int8_f32<3>(w), int8_f32<2>(w), 0x07060302u)};
 }
 
 // Four codes of format FMT to two dwords of exact fp16 (BF: bf16).

@@ -19,7 +19,7 @@
 // queries are brought into fp16's range by one power of two per row (elements
 // 2^29 below their row's largest lose bits). Key scales multiply the float32
 // scores. Value scales join the exponent: with s' = s + log2(scale) the weights
-// exp2(s' - M), M the running maximum of s' less W_SHIFT, are at most 2^14
+// exp2(s' - M), M the running maximum of s' less 13, are at most 2^13
 // whatever the scales, and are rounded to fp16 for the product (2^-11 relative); the sum l of
 // exp2(s - m) has its own maximum m. 16-bit tiles of bf16 take the weights as
 // two bf16 parts.
@@ -93,7 +93,7 @@ struct Decode {
     float mx = s[0];
 #pragma unroll
     for (int i = 1; i < N; ++i) mx = fmaxf(mx, s[i]);
-    const float Mn = fmaxf(M, lanes_max<16>(TWO ? mx + lv : mx) - W_SHIFT);
+    const float Mn = fmaxf(M, lanes_max<16>(TWO ? mx + lv : mx) - W_SHIFT<!TWO && BF>);
     const float ref = Mn == -INFINITY ? 0.f : Mn;
     if (__any(Mn > M)) {
       const float a = __builtin_amdgcn_exp2f(M - ref);
