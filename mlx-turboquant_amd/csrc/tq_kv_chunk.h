@@ -48,50 +48,51 @@ struct Chunk {
   static __device__ int krow(int t) { return (t & ~12) | (t & 4) << 1 | (t & 8) >> 1; }
 
   // ------------------------------------------------------- a tile of codes
-  __device__ void load8(const uint8_t* kc, const uint8_t* vc, int tile) {
-    const u4* k = (const u4*)(kc + (int64_t)tile * (TILE * D));
-    const u4* v = (const u4*)(vc + (int64_t)tile * (TILE * D));
+  static constexpr int PIECES = TILE * D / 16;
+  static constexpr bool EVEN = PIECES % CH_THREADS == 0;
+
+  static __device__ void load8(u4 (&x)[NK], const uint8_t* codes, int tile) {
+    const u4* v = (const u4*)(codes + (int64_t)tile * (TILE * D));
+#pragma unroll
+    for (int j = 0; j < NK; ++j) x[j] = v[EVEN ? j * CH_THREADS + threadIdx.x : min(j * CH_THREADS + (int)threadIdx.x, PIECES - 1)];
+  }
+  static __device__ void put16(u4 x, uint16_t* d) {
+    const u2 a = codes4<FMT, BF>(x.x), b = codes4<FMT, BF>(x.y), e = codes4<FMT, BF>(x.z), f = codes4<FMT, BF>(x.w);
+    *(u4*)d = u4{a.x, a.y, b.x, b.y};
+    *(u4*)(d + 8) = u4{e.x, e.y, f.x, f.y};
+  }
+  __device__ void store_k8(uint16_t* kl) const {
 #pragma unroll
     for (int j = 0; j < NK; ++j) {
       const int i = j * CH_THREADS + threadIdx.x;
-      if (TILE * D / 16 % CH_THREADS == 0 || i < TILE * D / 16) kx[j] = k[i], vx[j] = v[i];
+      if (EVEN || i < PIECES) put16(kx[j], kl + krow(i / (D / 16)) * KP + i % (D / 16) * 16);
     }
   }
-  __device__ void store8(const Params& p, const float* vsc, int t0, int main_len, uint16_t* kl, uint16_t* vl) const {
+  // fp16: times `pw`, the powers of two of the tile's four groups of 16 tokens
+  __device__ void store_v8(const float (&pw)[4], uint16_t* vl) const {
 #pragma unroll
     for (int j = 0; j < NK; ++j) {
       const int i = j * CH_THREADS + threadIdx.x;
-      if (TILE * D / 16 % CH_THREADS != 0 && i >= TILE * D / 16) break;
-      const int t = i / (D / 16), c = i % (D / 16);
-      uint16_t* d = kl + krow(t) * KP + c * 16;
-      const u4 x = kx[j];
-      const u2 a = codes4<FMT, BF>(x.x), b = codes4<FMT, BF>(x.y), e = codes4<FMT, BF>(x.z), f = codes4<FMT, BF>(x.w);
-      *(u4*)d = u4{a.x, a.y, b.x, b.y};
-      *(u4*)(d + 8) = u4{e.x, e.y, f.x, f.y};
-    }
-#pragma unroll
-    for (int j = 0; j < NK; ++j) {
-      const int i = j * CH_THREADS + threadIdx.x;
-      if (TILE * D / 16 % CH_THREADS != 0 && i >= TILE * D / 16) break;
-      const int dim = i / (TILE / 16), c = i % (TILE / 16);
-      uint16_t* d = vl + dim * VP + c * 16;
-      const u4 x = vx[j];
-      const u2 a = codes4<FMT, BF>(x.x), b = codes4<FMT, BF>(x.y), e = codes4<FMT, BF>(x.z), f = codes4<FMT, BF>(x.w);
-      u4 lo = {a.x, a.y, b.x, b.y}, hi = {e.x, e.y, f.x, f.y};
-      if constexpr (!BF) {
-        const float s = value_power(vsc[(t0 + c * 16) >> p.block_shift]);
-        const h8 sc = {(_Float16)s, (_Float16)s, (_Float16)s, (_Float16)s, (_Float16)s, (_Float16)s, (_Float16)s, (_Float16)s};
-        lo = __builtin_bit_cast(u4, __builtin_bit_cast(h8, lo) * sc);
-        hi = __builtin_bit_cast(u4, __builtin_bit_cast(h8, hi) * sc);
+      if (!EVEN && i >= PIECES) break;
+      const int c = i % (TILE / 16);
+      uint16_t* d = vl + i / (TILE / 16) * VP + c * 16;
+      if constexpr (BF) {
+        put16(vx[j], d);
+      } else {
+        const u4 x = vx[j];
+        const u2 a = codes4<FMT, BF>(x.x), b = codes4<FMT, BF>(x.y), e = codes4<FMT, BF>(x.z), f = codes4<FMT, BF>(x.w);
+        const _Float16 s = (_Float16)(c & 2 ? c & 1 ? pw[3] : pw[2] : c & 1 ? pw[1] : pw[0]);
+        const h8 sc = {s, s, s, s, s, s, s, s};
+        *(u4*)d = __builtin_bit_cast(u4, __builtin_bit_cast(h8, u4{a.x, a.y, b.x, b.y}) * sc);
+        *(u4*)(d + 8) = __builtin_bit_cast(u4, __builtin_bit_cast(h8, u4{e.x, e.y, f.x, f.y}) * sc);
       }
-      *(u4*)d = lo;
-      *(u4*)(d + 8) = hi;
     }
-    if (t0 + TILE > main_len) {  // tokens not written yet: any bytes
-      for (int i = threadIdx.x; i < TILE * D / 16; i += CH_THREADS) {
-        uint16_t* d = vl + i / (TILE / 16) * VP + i % (TILE / 16) * 16;
-        if (t0 + i % (TILE / 16) * 16 >= main_len) *(u4*)d = *(u4*)(d + 8) = u4{0, 0, 0, 0};
-      }
+  }
+  // values of tokens from `nv` on, which no write has reached: any bytes
+  static __device__ void clear_v8(int nv, uint16_t* vl) {
+    for (int i = threadIdx.x; i < PIECES; i += CH_THREADS) {
+      uint16_t* d = vl + i / (TILE / 16) * VP + i % (TILE / 16) * 16;
+      if (i % (TILE / 16) * 16 >= nv) *(u4*)d = *(u4*)(d + 8) = u4{0, 0, 0, 0};
     }
   }
 
@@ -107,36 +108,36 @@ struct Chunk {
   }
 
   // ------------------------------------------------- a tile of 16-bit tokens
-  // nv tokens at rows 0 .. of kb, vb; zeros after them. Values as 4 tokens x 8
-  // dims per thread, to be paired by tokens.
+  // nv tokens at rows 0 .. of kb, vb. Values as 4 tokens x 8 dims per thread, to
+  // be paired by tokens.
   static constexpr int KPIECES = TILE * D / 8, VTASKS = TILE / 4 * (D / 8);
+  // rows past nv repeat the last one: no weight reaches them
   static __device__ u4 k_piece(const uint16_t* kb, int64_t kst, int nv, int i) {
-    const int t = i / (D / 8), c = i % (D / 8);
-    return i < KPIECES && t < nv ? *(const u4*)(kb + (int64_t)t * kst + c * 8) : u4{0, 0, 0, 0};
+    return *(const u4*)(kb + min(i / (D / 8), nv - 1) * kst + i % (D / 8) * 8);
   }
   static __device__ void k_put(u4 x, int i, uint16_t* kl) {
     if (KPIECES % CH_THREADS == 0 || i < KPIECES) *(u4*)(kl + krow(i / (D / 8)) * KP + i % (D / 8) * 8) = x;
   }
   static __device__ u4 v_piece(const uint16_t* vb, int64_t vst, int nv, int i, int u) {
-    const int c = i % (D / 8), t = i / (D / 8) * 4 + u;
-    return i < VTASKS && t < nv ? *(const u4*)(vb + (int64_t)t * vst + c * 8) : u4{0, 0, 0, 0};
+    return *(const u4*)(vb + min(i / (D / 8) * 4 + u, nv - 1) * vst + i % (D / 8) * 8);
   }
-  // Infinite and NaN values go in as 0; returns whether there were any. MARKS:
-  // their marks go in, and 0 for the others.
-  template <bool MARKS>
-  static __device__ bool v_put(u4 (&x)[4], int i, uint16_t* vl) {
-    if (VTASKS % CH_THREADS != 0 && i >= VTASKS) return false;
+  // FINITE: infinite and NaN values go in as 0; MARKS: their marks go in, and 0
+  // for the others. Returns odd16() of the values.
+  enum { AS_IS, FINITE, MARKS };
+  template <int HOW>
+  static __device__ uint32_t v_put(const u4 (&v)[4], int i, uint16_t* vl) {
+    if (VTASKS % CH_THREADS != 0 && i >= VTASKS) return 0;
     const int c = i % (D / 8), t = i / (D / 8) * 4;
     uint32_t odd = 0;
+    u4 x[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < 4; ++u) {
+      x[u] = v[u];
 #pragma unroll
       for (int k = 0; k < 4; ++k) odd |= odd16<BF>(x[u][k]);
-    if (MARKS || odd & ODD_BITS) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      if (HOW != AS_IS) {
         const u4 mk = marks<BF>(x[u]);
-        if (MARKS) x[u] = mk;
+        if (HOW == MARKS) x[u] = mk;
       }
     }
 #pragma unroll
@@ -145,36 +146,36 @@ struct Chunk {
       *(u2*)(vl + (c * 8 + k) * VP + t) =
           u2{__builtin_amdgcn_perm(x[1][k / 2], x[0][k / 2], sel), __builtin_amdgcn_perm(x[3][k / 2], x[2][k / 2], sel)};
     }
-    return odd & ODD_BITS;
+    return odd;
   }
-  __device__ void load16(const uint16_t* kb, int64_t kst, const uint16_t* vb, int64_t vst, int nv) {
+  __device__ void load_k16(const uint16_t* kb, int64_t kst, int nv) {
 #pragma unroll
     for (int j = 0; j < NK; ++j) kx[j] = k_piece(kb, kst, nv, j * CH_THREADS + threadIdx.x);
+  }
+  __device__ void load_v16(const uint16_t* vb, int64_t vst, int nv) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) vx[j] = v_piece(vb, vst, nv, j / 4 * CH_THREADS + threadIdx.x, j % 4);
   }
-  __device__ bool store16(uint16_t* kl, uint16_t* vl) const {
-    bool odd = false;
+  __device__ void store_k16(uint16_t* kl) const {
 #pragma unroll
     for (int j = 0; j < NK; ++j) k_put(kx[j], j * CH_THREADS + threadIdx.x, kl);
+  }
+  template <int HOW>
+  __device__ uint32_t store_v16(uint16_t* vl) const {
+    uint32_t odd = 0;
 #pragma unroll
-    for (int j = 0; j < NV; j += 4) {
-      u4 x[4] = {vx[j], vx[j + 1], vx[j + 2], vx[j + 3]};
-      odd |= v_put<false>(x, j / 4 * CH_THREADS + threadIdx.x, vl);
-    }
+    for (int j = 0; j < NV; j += 4) odd |= v_put<HOW>({vx[j], vx[j + 1], vx[j + 2], vx[j + 3]}, j / 4 * CH_THREADS + threadIdx.x, vl);
     return odd;
   }
   // at once: the tail of an 8-bit cache, or any tile's marks (no keys)
-  template <bool MARKS>
+  template <int HOW>
   static __device__ bool stage16(const uint16_t* kb, int64_t kst, const uint16_t* vb, int64_t vst, int nv, uint16_t* kl, uint16_t* vl) {
-    bool odd = false;
-    if (!MARKS)
+    uint32_t odd = 0;
+    if (HOW != MARKS)
       for (int i = threadIdx.x; i < KPIECES; i += CH_THREADS) k_put(k_piece(kb, kst, nv, i), i, kl);
-    for (int i = threadIdx.x; i < VTASKS; i += CH_THREADS) {
-      u4 x[4] = {v_piece(vb, vst, nv, i, 0), v_piece(vb, vst, nv, i, 1), v_piece(vb, vst, nv, i, 2), v_piece(vb, vst, nv, i, 3)};
-      odd |= v_put<MARKS>(x, i, vl);
-    }
-    return odd;
+    for (int i = threadIdx.x; i < VTASKS; i += CH_THREADS)
+      odd |= v_put<HOW>({v_piece(vb, vst, nv, i, 0), v_piece(vb, vst, nv, i, 1), v_piece(vb, vst, nv, i, 2), v_piece(vb, vst, nv, i, 3)}, i, vl);
+    return odd & ODD_BITS;
   }
 };
 
@@ -211,7 +212,6 @@ __global__ __launch_bounds__(CH_THREADS, D > 128 ? 1 : 2) void chunk_kernel(cons
   // the wave's own span of positions
   const int wpmin = len - p.n_q + (row0 + wave * 32) / p.group;
   const int wpmax = min(pmax, len - p.n_q + (row0 + wave * 32 + 31) / p.group);
-  const bool wave_live = row0 + wave * 32 < p.rows;
 
   const uint8_t *kc = nullptr, *vc = nullptr;
   const float *ksc = nullptr, *vsc = nullptr;
@@ -227,18 +227,6 @@ __global__ __launch_bounds__(CH_THREADS, D > 128 ? 1 : 2) void chunk_kernel(cons
     kb = (const uint16_t*)p.k.p + (int64_t)b * p.k.sb + (int64_t)h * p.k.sh;
     vb = (const uint16_t*)p.v.p + (int64_t)b * p.v.sb + (int64_t)h * p.v.sh;
   }
-
-  C c;
-  // a tile's memory into registers (not the tail of an 8-bit cache)
-  const auto load = [&](int it) {
-    if (it >= last || it >= tl.n_main) return;
-    const int tile = tl.at(it);
-    if constexpr (CACHED)
-      c.load8(kc, vc, tile);
-    else
-      c.load16(kb + (int64_t)tile * TILE * p.k.st, p.k.st, vb + (int64_t)tile * TILE * p.v.st, p.v.st, len - tile * TILE);
-  };
-  load(first);
 
   // scores of a positive scale: their maximum is taken before it multiplies
   const float scale = p.scale == 0.f ? 1.f : fabsf(p.scale);
@@ -258,73 +246,51 @@ __global__ __launch_bounds__(CH_THREADS, D > 128 ? 1 : 2) void chunk_kernel(cons
   float m = -INFINITY, l = 0.f;
   bool odd = false;  // this thread met an infinite or NaN value
 
-  for (int it = first, buf = 0; it < last; ++it, buf ^= 1) {
-    uint16_t *kl = lds + buf * C::BUF, *vl = kl + TILE * C::KP;
-    const bool codes = CACHED && it < tl.n_main;
-    const int t0 = codes || !CACHED ? tl.at(it) * TILE : tl.main_len;
-    const int nv = min(TILE, (codes ? tl.main_len : len) - t0);
-    // 16 tokens each: what multiplies scores, log2 of what multiplies weights,
-    // and its inverse for their sum (a scale of 0 has codes of 0 only: 1 will do)
+  // What 16 tokens of codes each have: sc multiplies scores, lf is log2 of what
+  // multiplies weights, rf its inverse for their sum (a scale of 0 has codes of 0
+  // only: 1 will do).
+  struct Scales {
     float sc[4], lf[4], rf[4];
+  };
+  const auto scales_of = [&](int t0, bool codes) {
+    Scales x;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      sc[g] = scale, lf[g] = 0.f, rf[g] = 1.f;
+      x.sc[g] = scale, x.lf[g] = 0.f, x.rf[g] = 1.f;
       if (codes) {
         const int blk = (t0 + 16 * g) >> p.block_shift;
         const float ks = ksc[blk], f = C::value_factor(vsc[blk]);
-        sc[g] = ks == 0.f ? scale : scale * ks;
-        lf[g] = __builtin_amdgcn_logf(f);
-        rf[g] = f == f ? __builtin_amdgcn_rcpf(f) : 1.f;
+        x.sc[g] = ks == 0.f ? scale : scale * ks;
+        x.lf[g] = __builtin_amdgcn_logf(f);
+        x.rf[g] = f == f ? __builtin_amdgcn_rcpf(f) : 1.f;
       }
     }
-    if constexpr (CACHED) {
-      if (codes)
-        c.store8(p, vsc, t0, tl.main_len, kl, vl);
-      else
-        odd |= C::template stage16<false>(kb, D, vb, D, nv, kl, vl);
-    } else {
-      odd |= c.store16(kl, vl);
-    }
-    load(it + 1);
-    // One barrier per tile: a wave that is past it writes the other buffer, which
-    // everyone has read before coming here.
-    __syncthreads();
-    // nothing of the tile is seen by this wave
-    if (!wave_live || t0 > wpmax || (p.window && t0 + TILE - 1 <= wpmin - p.window && t0 >= p.sinks)) continue;
-
-    // scores
-    f16v s[2];
-#pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-#pragma unroll
-      for (int k = 0; k < 16; ++k) s[sub][k] = 0.f;
-      const uint16_t* kp = kl + (sub * 32 + n) * C::KP + hf * 8;
-#pragma unroll
-      for (int i = 0; i < NS; ++i) s[sub] = mma32<BF>(*(const u4*)(kp + i * 16), q[i], s[sub]);
-    }
-    const bool masked = nv < TILE || t0 + TILE - 1 > wpmin || (p.window && t0 <= wpmax - p.window && t0 + TILE > p.sinks);
-    if (masked) {
+    return x;
+  };
+  // Hides what the rows do not see of tokens t0 .. t0 + nv - 1 and moves the
+  // reference m where it has to.
+  const auto before = [&](f16v (&s)[2], Scales& x, int t0, int nv) {
+    if (nv < TILE || t0 + TILE - 1 > wpmin || (p.window && t0 <= wpmax - p.window && t0 + TILE > p.sinks)) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const uint32_t seen = seen_bits(t0 + 16 * g + 8 * hf, 8, t0 + nv, pos, low, p.sinks);
         // a block without a finite scale: NaN where it is seen only
-        const float bad = sc[g] + lf[g], nan = bad == bad ? 0.f : bad;
-        if (bad != bad) sc[g] = scale, lf[g] = 0.f;
+        const float bad = x.sc[g] + x.lf[g], nan = bad == bad ? 0.f : bad;
+        if (bad != bad) x.sc[g] = scale, x.lf[g] = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float x = s[g >> 1][(g & 1) * 8 + k] + nan;
-          s[g >> 1][(g & 1) * 8 + k] = seen >> k & 1 ? x : -INFINITY;
+          const float y = s[g >> 1][(g & 1) * 8 + k] + nan;
+          s[g >> 1][(g & 1) * 8 + k] = seen >> k & 1 ? y : -INFINITY;
         }
       }
     }
-    // softmax
     float top = -INFINITY;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      float x = s[g >> 1][(g & 1) * 8];
+      float y = s[g >> 1][(g & 1) * 8];
 #pragma unroll
-      for (int k = 1; k < 8; ++k) x = fmaxf(x, s[g >> 1][(g & 1) * 8 + k]);
-      top = fmaxf(top, x * sc[g]);
+      for (int k = 1; k < 8; ++k) y = fmaxf(y, s[g >> 1][(g & 1) * 8 + k]);
+      top = fmaxf(top, y * x.sc[g]);
     }
     top = lanes_max<32>(top) - W_SHIFT<BF>;
     if (__any(top > m + W_SLACK<BF>)) {
@@ -335,28 +301,150 @@ __global__ __launch_bounds__(CH_THREADS, D > 128 ? 1 : 2) void chunk_kernel(cons
       l *= a;
       m = mn;
     }
-    const float ref = m == -INFINITY ? 0.f : m;
-    u4 pw[4];
+  };
+  // Weights of 16 tokens (8 of them this lane's).
+  const auto weights = [&](const f16v (&s)[2], const Scales& x, int g) {
+    const float off = x.lf[g] - (m == -INFINITY ? 0.f : m);
+    float w[8], sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      w[k] = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][(g & 1) * 8 + k], x.sc[g], off));
+      sum += w[k];
+    }
+    l = fmaf(sum, x.rf[g], l);
+    return u4{bits2<BF>(w[0], w[1]), bits2<BF>(w[2], w[3]), bits2<BF>(w[4], w[5]), bits2<BF>(w[6], w[7])};
+  };
+  // A tile's scores, with `beside` among them; operands are on their way from LDS
+  // during the products before.
+  const auto scores = [&](f16v (&s)[2], const uint16_t* kl, auto beside) {
+    const uint16_t* kp = kl + n * C::KP + hf * 8;
+    u4 f[2][4];  // two steps of both halves
+    const auto read = [&](u4 (&f)[4], int i) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f[k] = *(const u4*)(kp + k % 2 * 32 * C::KP + (i + k / 2) * 16);
+    };
+    read(f[0], 0);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s[0][k] = s[1][k] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NS; i += 2) {
+      if (i + 2 < NS) read(f[i / 2 + 1 & 1], i + 2);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[k % 2] = mma32<BF>(f[i / 2 & 1][k], q[i + k / 2], s[k % 2]);
+      beside(i / 2);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // A tile's part of the output: the products of 16 tokens while the next 16
+  // weights are computed.
+  const auto output = [&](const f16v (&s)[2], const Scales& x, const uint16_t* vl) {
+    const uint16_t* vp = vl + n * C::VP + hf * 8;
+    u4 f[2][NO];
+    const auto read = [&](u4 (&f)[NO], int g) {
+#pragma unroll
+      for (int i = 0; i < NO; ++i) f[i] = *(const u4*)(vp + i * 32 * C::VP + g * 16);
+    };
+    read(f[0], 0);
+    u4 w = weights(s, x, 0);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      float w[8], sum = 0.f;
-      const float off = lf[g] - ref;
+      if (g < 3) read(f[g + 1 & 1], g + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float x = s[g >> 1][(g & 1) * 8 + k];
-        w[k] = __builtin_amdgcn_exp2f(fmaf(x, sc[g], off));
-        sum += w[k];
+      for (int i = 0; i < NO; ++i) o[i] = mma32<BF>(f[g & 1][i], w, o[i]);
+      if (g < 3) w = weights(s, x, g + 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  // The tiles but the tail of an 8-bit cache, j = 0 .. count - 1. While step j
+  // computes tile j's scores, tile j + 1 goes to LDS and tile j + 2 comes from
+  // memory. Past the last tile that happens with the last one again, for nobody.
+  // One barrier per step: what a step writes to LDS the step before has read.
+  const int count = min(last, tl.n_main) - first;
+  if (count > 0) {
+    C c;
+    const auto tile_at = [&](int j) { return tl.at(first + min(j, count - 1)); };
+    const auto load_k = [&](int j) {
+      const int t = tile_at(j);
+      if constexpr (CACHED)
+        C::load8(c.kx, kc, t);
+      else
+        c.load_k16(kb + (int64_t)t * TILE * p.k.st, p.k.st, len - t * TILE);
+    };
+    const auto load_v = [&](int j) {
+      const int t = tile_at(j);
+      if constexpr (CACHED)
+        C::load8(c.vx, vc, t);
+      else
+        c.load_v16(vb + (int64_t)t * TILE * p.v.st, p.v.st, len - t * TILE);
+    };
+    const auto k_at = [&](int j) { return lds + (j & 1) * C::BUF; };
+    const auto v_at = [&](int j) { return lds + (j & 1) * C::BUF + TILE * C::KP; };
+    const auto store_k = [&](int j) {
+      if constexpr (CACHED)
+        c.store_k8(k_at(j));
+      else
+        c.store_k16(k_at(j));
+    };
+    const auto store_v = [&](int j) {
+      uint32_t found = 0;
+      if constexpr (CACHED) {
+        float pw[4];
+        if constexpr (!BF)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) pw[g] = C::value_power(vsc[(tile_at(j) * TILE + 16 * g) >> p.block_shift]);
+        c.store_v8(pw, v_at(j));
+      } else {
+        found = c.template store_v16<C::AS_IS>(v_at(j));
       }
-      l = fmaf(sum, rf[g], l);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) pw[g][k] = bits2<BF>(w[2 * k], w[2 * k + 1]);
+      return found;
+    };
+    // what store_v left: apart from its straight line of code
+    const auto mend_v = [&](int j, uint32_t found) {
+      if constexpr (CACHED) {
+        const int nv = tl.main_len - tile_at(j) * TILE;
+        if (nv < TILE) C::clear_v8(nv, v_at(j));
+      } else if (found & ODD_BITS) {
+        odd = true;
+        c.template store_v16<C::FINITE>(v_at(j));
+      }
+    };
+    load_k(0);
+    load_v(0);
+    store_k(0);
+    load_k(1);
+    mend_v(0, store_v(0));
+    load_v(1);
+    for (int j = 0; j < count; ++j) {
+      const int t0 = tile_at(j) * TILE;
+      Scales x = scales_of(t0, CACHED);
+      __syncthreads();
+      f16v s[2];
+      uint32_t found = 0;
+      scores(s, k_at(j), [&](int i) {
+        if (i == 0) store_k(j + 1);
+        if (i == NS / 4) found = store_v(j + 1);
+      });
+      load_k(j + 2);
+      mend_v(j + 1, found);
+      load_v(j + 2);
+      before(s, x, t0, (CACHED ? tl.main_len : len) - t0);
+      output(s, x, v_at(j));
     }
-#pragma unroll
-    for (int i = 0; i < NO; ++i) {
-      const uint16_t* vp = vl + (i * 32 + n) * C::VP + hf * 8;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) o[i] = mma32<BF>(*(const u4*)(vp + g * 16), pw[g], o[i]);
-    }
+    __syncthreads();
+  }
+  if (CACHED && last > tl.n_main) {  // the tail
+    const int nv = len - tl.main_len;
+    uint16_t* vl = lds + TILE * C::KP;
+    odd |= C::template stage16<C::FINITE>(kb, D, vb, D, nv, lds, vl);
+    __syncthreads();
+    f16v s[2];
+    scores(s, lds, [](int) {});
+    Scales x = scales_of(tl.main_len, false);
+    before(s, x, tl.main_len, nv);
+    output(s, x, vl);
   }
 
   // Infinite and NaN values, left out so far: what the rows that see them get.
@@ -365,7 +453,7 @@ __global__ __launch_bounds__(CH_THREADS, D > 128 ? 1 : 2) void chunk_kernel(cons
       const int t0 = CACHED ? tl.main_len : tl.at(it) * TILE;
       const int nv = min(TILE, len - t0);
       const uint16_t* vt = CACHED ? vb : vb + (int64_t)t0 * p.v.st;
-      const bool some = C::template stage16<true>(nullptr, 0, vt, CACHED ? (int64_t)D : p.v.st, nv, nullptr, lds);
+      const bool some = C::template stage16<C::MARKS>(nullptr, 0, vt, CACHED ? (int64_t)D : p.v.st, nv, nullptr, lds);
       if (__syncthreads_or(some)) {
         u4 ones[4];
 #pragma unroll
