@@ -109,12 +109,17 @@ __device__ inline uint32_t bits2(float a, float b) {
 // and counted in one of their own, marks x seen: 1 for inf, 128 for -inf, 2^14
 // for NaN (at most 64 of each per tile: exact), which gives back what the rows
 // that see them get.
-// Bits 15 and 31: the exponent of that half is all ones (adding one to it carries).
-template <bool BF>
-__device__ inline uint32_t odd16(uint32_t x) {
-  return (x & 0x7fff7fffu) + (BF ? 0x00800080u : 0x04000400u);
+// The larger of two pairs of 16-bit magnitudes (signs off), half by half; whether
+// either is that of an infinity or NaN.
+__device__ inline uint32_t top16(uint32_t a, uint32_t x) {
+  typedef uint16_t s2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(s2, a), __builtin_bit_cast(s2, x & 0x7fff7fffu)));
 }
-constexpr uint32_t ODD_BITS = 0x80008000u;
+template <bool BF>
+__device__ inline bool odd16(uint32_t top) {
+  constexpr uint32_t ex = BF ? 0x7f80u : 0x7c00u;
+  return (top & 0xffffu) >= ex || top >> 16 >= ex;
+}
 template <bool BF>
 __device__ inline uint32_t mark16(uint32_t h) {
   constexpr uint32_t ex = BF ? 0x7f80u : 0x7c00u;

@@ -61,31 +61,25 @@ struct Chunk {
     *(u4*)d = u4{a.x, a.y, b.x, b.y};
     *(u4*)(d + 8) = u4{e.x, e.y, f.x, f.y};
   }
-  __device__ void store_k8(uint16_t* kl) const {
-#pragma unroll
-    for (int j = 0; j < NK; ++j) {
-      const int i = j * CH_THREADS + threadIdx.x;
-      if (EVEN || i < PIECES) put16(kx[j], kl + krow(i / (D / 16)) * KP + i % (D / 16) * 16);
-    }
+  __device__ void store_k8(uint16_t* kl, int j) const {
+    const int i = j * CH_THREADS + threadIdx.x;
+    if (EVEN || i < PIECES) put16(kx[j], kl + krow(i / (D / 16)) * KP + i % (D / 16) * 16);
   }
   // fp16: times `pw`, the powers of two of the tile's four groups of 16 tokens
-  __device__ void store_v8(const float (&pw)[4], uint16_t* vl) const {
-#pragma unroll
-    for (int j = 0; j < NK; ++j) {
-      const int i = j * CH_THREADS + threadIdx.x;
-      if (!EVEN && i >= PIECES) break;
-      const int c = i % (TILE / 16);
-      uint16_t* d = vl + i / (TILE / 16) * VP + c * 16;
-      if constexpr (BF) {
-        put16(vx[j], d);
-      } else {
-        const u4 x = vx[j];
-        const u2 a = codes4<FMT, BF>(x.x), b = codes4<FMT, BF>(x.y), e = codes4<FMT, BF>(x.z), f = codes4<FMT, BF>(x.w);
-        const _Float16 s = (_Float16)(c & 2 ? c & 1 ? pw[3] : pw[2] : c & 1 ? pw[1] : pw[0]);
-        const h8 sc = {s, s, s, s, s, s, s, s};
-        *(u4*)d = __builtin_bit_cast(u4, __builtin_bit_cast(h8, u4{a.x, a.y, b.x, b.y}) * sc);
-        *(u4*)(d + 8) = __builtin_bit_cast(u4, __builtin_bit_cast(h8, u4{e.x, e.y, f.x, f.y}) * sc);
-      }
+  __device__ void store_v8(const float (&pw)[4], uint16_t* vl, int j) const {
+    const int i = j * CH_THREADS + threadIdx.x;
+    if (!EVEN && i >= PIECES) return;
+    const int c = i % (TILE / 16);
+    uint16_t* d = vl + i / (TILE / 16) * VP + c * 16;
+    if constexpr (BF) {
+      put16(vx[j], d);
+    } else {
+      const u4 x = vx[j];
+      const u2 a = codes4<FMT, BF>(x.x), b = codes4<FMT, BF>(x.y), e = codes4<FMT, BF>(x.z), f = codes4<FMT, BF>(x.w);
+      const _Float16 s = (_Float16)(c & 2 ? c & 1 ? pw[3] : pw[2] : c & 1 ? pw[1] : pw[0]);
+      const h8 sc = {s, s, s, s, s, s, s, s};
+      *(u4*)d = __builtin_bit_cast(u4, __builtin_bit_cast(h8, u4{a.x, a.y, b.x, b.y}) * sc);
+      *(u4*)(d + 8) = __builtin_bit_cast(u4, __builtin_bit_cast(h8, u4{e.x, e.y, f.x, f.y}) * sc);
     }
   }
   // values of tokens from `nv` on, which no write has reached: any bytes
@@ -122,19 +116,19 @@ struct Chunk {
     return *(const u4*)(vb + min(i / (D / 8) * 4 + u, nv - 1) * vst + i % (D / 8) * 8);
   }
   // FINITE: infinite and NaN values go in as 0; MARKS: their marks go in, and 0
-  // for the others. Returns odd16() of the values.
+  // for the others. Returns top16() of the values.
   enum { AS_IS, FINITE, MARKS };
   template <int HOW>
   static __device__ uint32_t v_put(const u4 (&v)[4], int i, uint16_t* vl) {
     if (VTASKS % CH_THREADS != 0 && i >= VTASKS) return 0;
     const int c = i % (D / 8), t = i / (D / 8) * 4;
-    uint32_t odd = 0;
+    uint32_t top = 0;
     u4 x[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       x[u] = v[u];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) odd |= odd16<BF>(x[u][k]);
+      for (int k = 0; k < 4; ++k) top = top16(top, x[u][k]);
       if (HOW != AS_IS) {
         const u4 mk = marks<BF>(x[u]);
         if (HOW == MARKS) x[u] = mk;
@@ -146,36 +140,51 @@ struct Chunk {
       *(u2*)(vl + (c * 8 + k) * VP + t) =
           u2{__builtin_amdgcn_perm(x[1][k / 2], x[0][k / 2], sel), __builtin_amdgcn_perm(x[3][k / 2], x[2][k / 2], sel)};
     }
-    return odd;
+    return top;
+  }
+  // A thread's pieces are whole rows apart (D = 96: not): its own offset, and
+  // uniform ones.
+  static constexpr int ROWS = CH_THREADS / (D / 8);
+  static constexpr bool APART = CH_THREADS % (D / 8) == 0;
+  int64_t k_off, v_off;
+  __device__ void offsets(int64_t kst, int64_t vst) {
+    k_off = (int64_t)(threadIdx.x / (D / 8)) * kst + threadIdx.x % (D / 8) * 8;
+    v_off = (int64_t)(threadIdx.x / (D / 8)) * 4 * vst + threadIdx.x % (D / 8) * 8;
   }
   __device__ void load_k16(const uint16_t* kb, int64_t kst, int nv) {
+    if (APART && nv >= TILE) {
 #pragma unroll
-    for (int j = 0; j < NK; ++j) kx[j] = k_piece(kb, kst, nv, j * CH_THREADS + threadIdx.x);
+      for (int j = 0; j < NK; ++j) kx[j] = *(const u4*)(kb + j * ROWS * kst + k_off);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NK; ++j) kx[j] = k_piece(kb, kst, nv, j * CH_THREADS + threadIdx.x);
+    }
   }
   __device__ void load_v16(const uint16_t* vb, int64_t vst, int nv) {
+    if (APART && VTASKS % CH_THREADS == 0 && nv >= TILE) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) vx[j] = v_piece(vb, vst, nv, j / 4 * CH_THREADS + threadIdx.x, j % 4);
-  }
-  __device__ void store_k16(uint16_t* kl) const {
+      for (int j = 0; j < NV; ++j) vx[j] = *(const u4*)(vb + (j / 4 * ROWS * 4 + j % 4) * vst + v_off);
+    } else {
 #pragma unroll
-    for (int j = 0; j < NK; ++j) k_put(kx[j], j * CH_THREADS + threadIdx.x, kl);
+      for (int j = 0; j < NV; ++j) vx[j] = v_piece(vb, vst, nv, j / 4 * CH_THREADS + threadIdx.x, j % 4);
+    }
   }
+  __device__ void store_k16(uint16_t* kl, int j) const { k_put(kx[j], j * CH_THREADS + threadIdx.x, kl); }
   template <int HOW>
-  __device__ uint32_t store_v16(uint16_t* vl) const {
-    uint32_t odd = 0;
-#pragma unroll
-    for (int j = 0; j < NV; j += 4) odd |= v_put<HOW>({vx[j], vx[j + 1], vx[j + 2], vx[j + 3]}, j / 4 * CH_THREADS + threadIdx.x, vl);
-    return odd;
+  __device__ uint32_t store_v16(uint16_t* vl, int j) const {
+    return v_put<HOW>({vx[4 * j], vx[4 * j + 1], vx[4 * j + 2], vx[4 * j + 3]}, j * CH_THREADS + threadIdx.x, vl);
   }
+  // pieces of a thread's part of a tile to LDS
+  static constexpr int PK = NK, PV = CACHED ? NK : NV / 4;
   // at once: the tail of an 8-bit cache, or any tile's marks (no keys)
   template <int HOW>
   static __device__ bool stage16(const uint16_t* kb, int64_t kst, const uint16_t* vb, int64_t vst, int nv, uint16_t* kl, uint16_t* vl) {
-    uint32_t odd = 0;
+    uint32_t top = 0;
     if (HOW != MARKS)
       for (int i = threadIdx.x; i < KPIECES; i += CH_THREADS) k_put(k_piece(kb, kst, nv, i), i, kl);
     for (int i = threadIdx.x; i < VTASKS; i += CH_THREADS)
-      odd |= v_put<HOW>({v_piece(vb, vst, nv, i, 0), v_piece(vb, vst, nv, i, 1), v_piece(vb, vst, nv, i, 2), v_piece(vb, vst, nv, i, 3)}, i, vl);
-    return odd & ODD_BITS;
+      top = top16(top, v_put<HOW>({v_piece(vb, vst, nv, i, 0), v_piece(vb, vst, nv, i, 1), v_piece(vb, vst, nv, i, 2), v_piece(vb, vst, nv, i, 3)}, i, vl));
+    return odd16<BF>(top);
   }
 };
 
@@ -314,6 +323,14 @@ __global__ __launch_bounds__(CH_THREADS, D > 128 ? 1 : 2) void chunk_kernel(cons
     l = fmaf(sum, x.rf[g], l);
     return u4{bits2<BF>(w[0], w[1]), bits2<BF>(w[2], w[3]), bits2<BF>(w[4], w[5]), bits2<BF>(w[6], w[7])};
   };
+  // Other work goes between the products, a few instructions each: what runs
+  // under a product (they do not run beside another wave's).
+  const auto between = [](int n) {
+    for (int i = 0; i < n; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // MFMA
+      __builtin_amdgcn_sched_group_barrier(0x2, 7, 0);  // VALU
+    }
+  };
   // A tile's scores, with `beside` among them; operands are on their way from LDS
   // during the products before.
   const auto scores = [&](f16v (&s)[2], const uint16_t* kl, auto beside) {
@@ -333,6 +350,7 @@ __global__ __launch_bounds__(CH_THREADS, D > 128 ? 1 : 2) void chunk_kernel(cons
 #pragma unroll
       for (int k = 0; k < 4; ++k) s[k % 2] = mma32<BF>(f[i / 2 & 1][k], q[i + k / 2], s[k % 2]);
       beside(i / 2);
+      between(4);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -354,6 +372,7 @@ __global__ __launch_bounds__(CH_THREADS, D > 128 ? 1 : 2) void chunk_kernel(cons
 #pragma unroll
       for (int i = 0; i < NO; ++i) o[i] = mma32<BF>(f[g & 1][i], w, o[i]);
       if (g < 3) w = weights(s, x, g + 1);
+      between(NO);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -365,6 +384,7 @@ __global__ __launch_bounds__(CH_THREADS, D > 128 ? 1 : 2) void chunk_kernel(cons
   const int count = min(last, tl.n_main) - first;
   if (count > 0) {
     C c;
+    if constexpr (!CACHED) c.offsets(p.k.st, p.v.st);
     const auto tile_at = [&](int j) { return tl.at(first + min(j, count - 1)); };
     const auto load_k = [&](int j) {
       const int t = tile_at(j);
@@ -382,50 +402,59 @@ __global__ __launch_bounds__(CH_THREADS, D > 128 ? 1 : 2) void chunk_kernel(cons
     };
     const auto k_at = [&](int j) { return lds + (j & 1) * C::BUF; };
     const auto v_at = [&](int j) { return lds + (j & 1) * C::BUF + TILE * C::KP; };
-    const auto store_k = [&](int j) {
-      if constexpr (CACHED)
-        c.store_k8(k_at(j));
-      else
-        c.store_k16(k_at(j));
-    };
-    const auto store_v = [&](int j) {
-      uint32_t found = 0;
+    // piece i of the C::PK + C::PV of tile j's keys and values
+    const auto store = [&](int j, int i, const float (&pw)[4]) -> uint32_t {
       if constexpr (CACHED) {
-        float pw[4];
-        if constexpr (!BF)
-#pragma unroll
-          for (int g = 0; g < 4; ++g) pw[g] = C::value_power(vsc[(tile_at(j) * TILE + 16 * g) >> p.block_shift]);
-        c.store_v8(pw, v_at(j));
+        if (i < C::PK)
+          c.store_k8(k_at(j), i);
+        else
+          c.store_v8(pw, v_at(j), i - C::PK);
+        return 0;
       } else {
-        found = c.template store_v16<C::AS_IS>(v_at(j));
+        if (i < C::PK) {
+          c.store_k16(k_at(j), i);
+          return 0;
+        }
+        return c.template store_v16<C::AS_IS>(v_at(j), i - C::PK);
       }
-      return found;
     };
-    // what store_v left: apart from its straight line of code
+    const auto powers = [&](int j, float (&pw)[4]) {
+      if constexpr (CACHED && !BF)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) pw[g] = C::value_power(vsc[(tile_at(j) * TILE + 16 * g) >> p.block_shift]);
+    };
+    // what store left: apart from its straight line of code
     const auto mend_v = [&](int j, uint32_t found) {
       if constexpr (CACHED) {
         const int nv = tl.main_len - tile_at(j) * TILE;
         if (nv < TILE) C::clear_v8(nv, v_at(j));
-      } else if (found & ODD_BITS) {
+      } else if (odd16<BF>(found)) {
         odd = true;
-        c.template store_v16<C::FINITE>(v_at(j));
+#pragma unroll
+        for (int i = 0; i < C::PV; ++i) c.template store_v16<C::FINITE>(v_at(j), i);
       }
     };
+    float pw[4];
+    uint32_t found = 0;
     load_k(0);
     load_v(0);
-    store_k(0);
+    powers(0, pw);
+#pragma unroll
+    for (int i = 0; i < C::PK + C::PV; ++i) found = top16(found, store(0, i, pw));
     load_k(1);
-    mend_v(0, store_v(0));
+    mend_v(0, found);
     load_v(1);
     for (int j = 0; j < count; ++j) {
       const int t0 = tile_at(j) * TILE;
       Scales x = scales_of(t0, CACHED);
       __syncthreads();
       f16v s[2];
-      uint32_t found = 0;
-      scores(s, k_at(j), [&](int i) {
-        if (i == 0) store_k(j + 1);
-        if (i == NS / 4) found = store_v(j + 1);
+      found = 0;
+      powers(j + 1, pw);
+      scores(s, k_at(j), [&](int r) {  // the pieces spread over the NS / 2 groups of products
+#pragma unroll
+        for (int i = 0; i < C::PK + C::PV; ++i)
+          if (i * (NS / 2) / (C::PK + C::PV) == r) found = top16(found, store(j + 1, i, pw));
       });
       load_k(j + 2);
       mend_v(j + 1, found);

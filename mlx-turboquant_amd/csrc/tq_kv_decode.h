@@ -283,14 +283,14 @@ struct Decode {
       pw[i] = bits2<BF>(w[2 * i], w[2 * i + 1]);
       if constexpr (BF) px[i] = bits2<true>(w[2 * i] - elem<true>(pw[i] & 0xffff), w[2 * i + 1] - elem<true>(pw[i] >> 16));
     }
-    uint32_t odd = 0;
+    uint32_t top = 0;
     if (masked) {
 #pragma unroll
       for (int u = 0; u < 8; ++u)
 #pragma unroll
-        for (int i = 0; i < NO / 2; ++i) odd |= odd16<BF>(v16[u][i]);
+        for (int i = 0; i < NO / 2; ++i) top = top16(top, v16[u][i]);
     }
-    const bool apart = __any(odd & ODD_BITS);
+    const bool apart = __any(odd16<BF>(top));
     const u4 ones = {seen2<BF>(seen), seen2<BF>(seen >> 2), seen2<BF>(seen >> 4), seen2<BF>(seen >> 6)};
 #pragma unroll
     for (int i = 0; i < NO; ++i) {
