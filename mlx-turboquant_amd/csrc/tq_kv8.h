@@ -23,7 +23,6 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr int TILE = 64;     // tokens per tile (and per transposed tile of value codes)
 constexpr int HALF = TILE / 2;
 constexpr int DEC_WAVES = 4, DEC_ROWS = 16;            // tq_kv_decode.h: waves and most rows per workgroup
-constexpr int CH_WAVES = 4, CH_ROWS = CH_WAVES * 32;   // tq_kv_chunk.h
 constexpr int DENSE = -1;    // format of uncompressed keys and values (else TQ_KV8_*)
 // The reference of the softmax's weights, in base 2: this far below the running
 // maximum. fp16 weights then reach 2^14, which leaves those down to 2^-28 of the
@@ -204,7 +203,7 @@ struct Params {
   int32_t max_len, block_shift, window, sinks;
   int32_t wgs;            // decode: workgroups that share the list of all tiles; 0: one per (sequence, kv head)
   int32_t splits, chunk;  // chunk kernel: a split is `chunk` consecutive tiles
-  int32_t row_tiles;      // chunk kernel: row tiles of a kv head
+  int32_t tile_rows, row_tiles;  // chunk kernel: rows per workgroup (128, 256), and how many such per kv head
   int32_t out_f32;
   float scale;            // times log2 e: scores are kept in base 2
 };

@@ -53,8 +53,8 @@ __global__ __launch_bounds__(MT) void merge_kernel(const Params p, bool cached) 
     slot = (int64_t)(at / sh.per + bh) * p.rows + row;
     step = p.rows;
   } else {
-    const int r0 = row / CH_ROWS * CH_ROWS;
-    const int pmin = len - p.n_q + r0 / p.group, pmax = len - p.n_q + min(p.rows - 1, r0 + CH_ROWS - 1) / p.group;
+    const int r0 = row / p.tile_rows * p.tile_rows;
+    const int pmin = len - p.n_q + r0 / p.group, pmax = len - p.n_q + min(p.rows - 1, r0 + p.tile_rows - 1) / p.group;
     count = (tiles_of(len, cached, p.block_shift, pmin, pmax, p.window, p.sinks).n + p.chunk - 1) / p.chunk;
     slot = (int64_t)unit * p.splits;
     step = 1;
@@ -138,18 +138,26 @@ int plan(const tq_kv8_store* s, const tq_kv_attn_desc* d, Params& p, bool& decod
   p.out_f32 = d->out_dtype == TQ_F32;
   p.scale = d->scale * 1.44269504088896340736f;
   decode = p.rows <= DEC_ROWS;
-  p.row_tiles = decode ? 1 : (p.rows + CH_ROWS - 1) / CH_ROWS;
-
+  const int64_t heads = (int64_t)p.batch * p.hkv;
   // tiles that a group of rows reads at most, the tail among them
-  int64_t tiles = ((int64_t)d->max_len + TILE - 1) / TILE;
-  if (p.window) {
-    const int64_t span = decode ? p.n_q : (p.n_q < CH_ROWS / p.group + 2 ? p.n_q : CH_ROWS / p.group + 2);
-    const int64_t w = (p.sinks + TILE - 1) / TILE + (p.window + span + TILE - 1) / TILE + 1;
-    tiles = w < tiles ? w : tiles;
-  }
-  tiles += s != nullptr;
-  if (tiles < 1) tiles = 1;
-  const int64_t units = (int64_t)p.batch * p.hkv, base = units * p.row_tiles;
+  const auto most_tiles = [&](int64_t rows) {
+    int64_t tiles = ((int64_t)d->max_len + TILE - 1) / TILE;
+    if (p.window) {
+      const int64_t span = std::min<int64_t>(p.n_q, rows / p.group + 2);
+      tiles = std::min<int64_t>(tiles, (p.sinks + TILE - 1) / TILE + (p.window + span + TILE - 1) / TILE + 1);
+    }
+    return std::max<int64_t>(1, tiles + (s != nullptr));
+  };
+  // Rows per workgroup of the chunk kernel. 256 (one workgroup of 8 waves per
+  // CU) share each tile's way through LDS among twice the rows, where they still
+  // fill the chip and have many tiles (8192 bf16 queries of 32 heads on 8, head
+  // dim 128: window 8192 1088 us against 1177 for 128, 2048 316 against 327);
+  // with few, two workgroups of 4 waves per CU hide each other's beginnings and
+  // ends (window 1024: 192 us against 197).
+  p.tile_rows = d->d <= 128 && heads * ((p.rows + 255) / 256) >= 256 && most_tiles(256) >= 32 ? 256 : 128;
+  p.row_tiles = decode ? 1 : (p.rows + p.tile_rows - 1) / p.tile_rows;
+  const int64_t tiles = most_tiles(decode ? p.rows : p.tile_rows);
+  const int64_t units = heads, base = units * p.row_tiles;
   if (base >= (int64_t)1 << 31 || units * p.rows >= (int64_t)1 << 31 || units * tiles >= (int64_t)1 << 30)
     return set_error(TQ_ERR_UNSUPPORTED, "attention: too many rows or tokens in one call");
   int64_t slots = 0;

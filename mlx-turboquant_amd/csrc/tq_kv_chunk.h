@@ -30,17 +30,18 @@
 namespace tq {
 namespace kv {
 
-constexpr int CH_THREADS = CH_WAVES * 64;
 
-template <int D, bool BF, int FMT>
+template <int D, bool BF, int FMT, int WAVES>
 struct Chunk {
+  static constexpr int CH_THREADS = WAVES * 64;
   static constexpr bool CACHED = FMT != DENSE;
   static constexpr int KP = D + 8, VP = TILE + 8;  // row pitches: reads of 16 lanes hit 64 banks
   static constexpr int BUF = TILE * KP + D * VP;   // elements of a tile's K and V
   static constexpr int LDS = 2 * BUF * 2;
   // what a thread loads of a tile: pieces of 16 codes, or of 8 elements
   static constexpr int NK = (TILE * D / (CACHED ? 16 : 8) + CH_THREADS - 1) / CH_THREADS;
-  static constexpr int NV = CACHED ? NK : (TILE / 4 * (D / 8) + CH_THREADS - 1) / CH_THREADS * 4;
+  static constexpr int VTOK = WAVES == 8 ? 2 : 4;  // 16-bit values: tokens that a thread pairs
+  static constexpr int NV = CACHED ? NK : (TILE / VTOK * (D / 8) + CH_THREADS - 1) / CH_THREADS * VTOK;
 
   u4 kx[NK], vx[NV];  // on their way from memory
 
@@ -90,21 +91,23 @@ struct Chunk {
     }
   }
 
-  // 2^e of the value scale that fp16 values carry: codes * 2^e stay in fp16's range
-  static __device__ float value_power(float s) {
-    if (!(s > 0.f)) return 1.f;
-    return ldexpf(1.f, min(max(ilogbf(s), -24), FMT == TQ_KV8_INT8 ? 9 : 7));
+  // e of the power of two of a value scale that fp16 values carry: codes * 2^e
+  // stay in fp16's range
+  static __device__ int value_exponent(float s) {
+    return min(max((int)(__float_as_uint(s) >> 23 & 255) - 127, -24), FMT == TQ_KV8_INT8 ? 9 : 7);
   }
+  static __device__ float value_power(float s) { return __uint_as_float((uint32_t)(127 + value_exponent(s)) << 23); }
   // what the weights carry (codes of a scale of 0 are 0: any weight will do)
   static __device__ float value_factor(float s) {
-    if (s == 0.f) return 1.f;
-    return BF ? s : s * (1.f / value_power(s));
+    const float f = BF ? s : s * __uint_as_float((uint32_t)(127 - value_exponent(s)) << 23);
+    return s == 0.f ? 1.f : f;
   }
 
   // ------------------------------------------------- a tile of 16-bit tokens
-  // nv tokens at rows 0 .. of kb, vb. Values as 4 tokens x 8 dims per thread, to
-  // be paired by tokens.
-  static constexpr int KPIECES = TILE * D / 8, VTASKS = TILE / 4 * (D / 8);
+  // nv tokens at rows 0 .. of kb, vb. Values as VTOK tokens x 8 dims per thread, to
+  // be paired by tokens; tokens go along the lanes, so that they meet LDS's banks
+  // in turn.
+  static constexpr int KPIECES = TILE * D / 8, VSPAN = TILE / VTOK, VTASKS = VSPAN * (D / 8);
   // rows past nv repeat the last one: no weight reaches them
   static __device__ u4 k_piece(const uint16_t* kb, int64_t kst, int nv, int i) {
     return *(const u4*)(kb + min(i / (D / 8), nv - 1) * kst + i % (D / 8) * 8);
@@ -113,19 +116,19 @@ struct Chunk {
     if (KPIECES % CH_THREADS == 0 || i < KPIECES) *(u4*)(kl + krow(i / (D / 8)) * KP + i % (D / 8) * 8) = x;
   }
   static __device__ u4 v_piece(const uint16_t* vb, int64_t vst, int nv, int i, int u) {
-    return *(const u4*)(vb + min(i / (D / 8) * 4 + u, nv - 1) * vst + i % (D / 8) * 8);
+    return *(const u4*)(vb + min(i % VSPAN * VTOK + u, nv - 1) * vst + i / VSPAN * 8);
   }
   // FINITE: infinite and NaN values go in as 0; MARKS: their marks go in, and 0
   // for the others. Returns top16() of the values.
   enum { AS_IS, FINITE, MARKS };
   template <int HOW>
-  static __device__ uint32_t v_put(const u4 (&v)[4], int i, uint16_t* vl) {
+  static __device__ uint32_t v_put(const u4 (&v)[VTOK], int i, uint16_t* vl) {
     if (VTASKS % CH_THREADS != 0 && i >= VTASKS) return 0;
-    const int c = i % (D / 8), t = i / (D / 8) * 4;
+    const int c = i / VSPAN, t = i % VSPAN * VTOK;
     uint32_t top = 0;
-    u4 x[4];
+    u4 x[VTOK];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < VTOK; ++u) {
       x[u] = v[u];
 #pragma unroll
       for (int k = 0; k < 4; ++k) top = top16(top, x[u][k]);
@@ -137,8 +140,12 @@ struct Chunk {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const uint32_t sel = k & 1 ? 0x07060302u : 0x05040100u;
-      *(u2*)(vl + (c * 8 + k) * VP + t) =
-          u2{__builtin_amdgcn_perm(x[1][k / 2], x[0][k / 2], sel), __builtin_amdgcn_perm(x[3][k / 2], x[2][k / 2], sel)};
+      const uint32_t lo = __builtin_amdgcn_perm(x[1][k / 2], x[0][k / 2], sel);
+      uint16_t* d = vl + (c * 8 + k) * VP + t;
+      if constexpr (VTOK == 4)
+        *(u2*)d = u2{lo, __builtin_amdgcn_perm(x[3][k / 2], x[2][k / 2], sel)};
+      else
+        *(uint32_t*)d = lo;
     }
     return top;
   }
@@ -149,7 +156,7 @@ struct Chunk {
   int64_t k_off, v_off;
   __device__ void offsets(int64_t kst, int64_t vst) {
     k_off = (int64_t)(threadIdx.x / (D / 8)) * kst + threadIdx.x % (D / 8) * 8;
-    v_off = (int64_t)(threadIdx.x / (D / 8)) * 4 * vst + threadIdx.x % (D / 8) * 8;
+    v_off = (int64_t)(threadIdx.x % VSPAN * VTOK) * vst + threadIdx.x / VSPAN * 8;
   }
   __device__ void load_k16(const uint16_t* kb, int64_t kst, int nv) {
     if (APART && nv >= TILE) {
@@ -161,36 +168,46 @@ struct Chunk {
     }
   }
   __device__ void load_v16(const uint16_t* vb, int64_t vst, int nv) {
-    if (APART && VTASKS % CH_THREADS == 0 && nv >= TILE) {
+    if (nv >= TILE) {
+      if (VTASKS % CH_THREADS == 0 || threadIdx.x < VTASKS) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) vx[j] = *(const u4*)(vb + (j / 4 * ROWS * 4 + j % 4) * vst + v_off);
+        for (int j = 0; j < NV; ++j) vx[j] = *(const u4*)(vb + j % VTOK * vst + v_off + j / VTOK * (CH_THREADS / VSPAN * 8));
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) vx[j] = v_piece(vb, vst, nv, j / 4 * CH_THREADS + threadIdx.x, j % 4);
+      for (int j = 0; j < NV; ++j) vx[j] = v_piece(vb, vst, nv, min(j / VTOK * CH_THREADS + (int)threadIdx.x, VTASKS - 1), j % VTOK);
     }
   }
   __device__ void store_k16(uint16_t* kl, int j) const { k_put(kx[j], j * CH_THREADS + threadIdx.x, kl); }
   template <int HOW>
   __device__ uint32_t store_v16(uint16_t* vl, int j) const {
-    return v_put<HOW>({vx[4 * j], vx[4 * j + 1], vx[4 * j + 2], vx[4 * j + 3]}, j * CH_THREADS + threadIdx.x, vl);
+    u4 x[VTOK];
+#pragma unroll
+    for (int u = 0; u < VTOK; ++u) x[u] = vx[VTOK * j + u];
+    return v_put<HOW>(x, j * CH_THREADS + threadIdx.x, vl);
   }
   // pieces of a thread's part of a tile to LDS
-  static constexpr int PK = NK, PV = CACHED ? NK : NV / 4;
+  static constexpr int PK = NK, PV = CACHED ? NK : NV / VTOK;
   // at once: the tail of an 8-bit cache, or any tile's marks (no keys)
   template <int HOW>
   static __device__ bool stage16(const uint16_t* kb, int64_t kst, const uint16_t* vb, int64_t vst, int nv, uint16_t* kl, uint16_t* vl) {
     uint32_t top = 0;
     if (HOW != MARKS)
       for (int i = threadIdx.x; i < KPIECES; i += CH_THREADS) k_put(k_piece(kb, kst, nv, i), i, kl);
-    for (int i = threadIdx.x; i < VTASKS; i += CH_THREADS)
-      top = top16(top, v_put<HOW>({v_piece(vb, vst, nv, i, 0), v_piece(vb, vst, nv, i, 1), v_piece(vb, vst, nv, i, 2), v_piece(vb, vst, nv, i, 3)}, i, vl));
+    for (int i = threadIdx.x; i < VTASKS; i += CH_THREADS) {
+      u4 x[VTOK];
+#pragma unroll
+      for (int u = 0; u < VTOK; ++u) x[u] = v_piece(vb, vst, nv, i, u);
+      top = top16(top, v_put<HOW>(x, i, vl));
+    }
     return odd16<BF>(top);
   }
 };
 
-template <int D, bool BF, int FMT>
-__global__ __launch_bounds__(CH_THREADS, D > 128 ? 1 : 2) void chunk_kernel(const Params p) {
-  using C = Chunk<D, BF, FMT>;
+template <int D, bool BF, int FMT, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(const Params p) {
+  using C = Chunk<D, BF, FMT, WAVES>;
+  constexpr int CH_ROWS = WAVES * 32;
   constexpr bool CACHED = FMT != DENSE;
   constexpr int NS = D / 16, NO = D / 32;
   extern __shared__ __align__(16) uint16_t lds[];
@@ -521,6 +538,7 @@ __global__ __launch_bounds__(CH_THREADS, D > 128 ? 1 : 2) void chunk_kernel(cons
     return;
   }
   const int64_t at = (int64_t)b * p.out.sb + (int64_t)(h * p.group + head) * p.out.sh + (int64_t)qi * p.out.st;
+  const float inv = 1.f / l;
 #pragma unroll
   for (int i = 0; i < NO; ++i)
 #pragma unroll
@@ -528,7 +546,7 @@ __global__ __launch_bounds__(CH_THREADS, D > 128 ? 1 : 2) void chunk_kernel(cons
       const int dim = i * 32 + k * 8 + hf * 4;
       f4 x;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = pos < 0 ? 0.f : o[i][4 * k + j] / l;
+      for (int j = 0; j < 4; ++j) x[j] = pos < 0 ? 0.f : o[i][4 * k + j] * inv;
       if (p.out_f32)
         *(f4*)((float*)p.out.p + at + dim) = x;
       else
@@ -536,25 +554,32 @@ __global__ __launch_bounds__(CH_THREADS, D > 128 ? 1 : 2) void chunk_kernel(cons
     }
 }
 
-template <int D, bool BF, int FMT>
+template <int D, bool BF, int FMT, int WAVES>
 hipError_t launch_chunk_as(const Params& p, hipStream_t stream) {
-  constexpr int bytes = Chunk<D, BF, FMT>::LDS;
-  static_assert(bytes + 16 <= 160 * 1024, "LDS");
-  auto kern = chunk_kernel<D, BF, FMT>;
+  constexpr int bytes = Chunk<D, BF, FMT, WAVES>::LDS;
+  static_assert(bytes <= 160 * 1024, "LDS");
+  auto kern = chunk_kernel<D, BF, FMT, WAVES>;
   if (bytes > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != hipSuccess) return e;
   }
-  kern<<<(uint32_t)(p.splits * p.row_tiles * p.batch * p.hkv), CH_THREADS, bytes, stream>>>(p);
+  kern<<<(uint32_t)(p.splits * p.row_tiles * p.batch * p.hkv), WAVES * 64, bytes, stream>>>(p);
   return hipGetLastError();
+}
+
+template <int D, bool BF>
+hipError_t launch_chunk_of(const Params& p, int fmt, hipStream_t stream) {
+  if constexpr (D <= 128)
+    if (p.tile_rows == 256)
+      return fmt == DENSE ? launch_chunk_as<D, BF, DENSE, 8>(p, stream)
+             : fmt == TQ_KV8_INT8 ? launch_chunk_as<D, BF, TQ_KV8_INT8, 8>(p, stream) : launch_chunk_as<D, BF, TQ_KV8_E4M3, 8>(p, stream);
+  return fmt == DENSE ? launch_chunk_as<D, BF, DENSE, 4>(p, stream)
+         : fmt == TQ_KV8_INT8 ? launch_chunk_as<D, BF, TQ_KV8_INT8, 4>(p, stream) : launch_chunk_as<D, BF, TQ_KV8_E4M3, 4>(p, stream);
 }
 
 template <int D>
 hipError_t launch_chunk(const Params& p, bool bf16, int fmt, hipStream_t stream) {
-  if (fmt == DENSE) return bf16 ? launch_chunk_as<D, true, DENSE>(p, stream) : launch_chunk_as<D, false, DENSE>(p, stream);
-  if (fmt == TQ_KV8_INT8)
-    return bf16 ? launch_chunk_as<D, true, TQ_KV8_INT8>(p, stream) : launch_chunk_as<D, false, TQ_KV8_INT8>(p, stream);
-  return bf16 ? launch_chunk_as<D, true, TQ_KV8_E4M3>(p, stream) : launch_chunk_as<D, false, TQ_KV8_E4M3>(p, stream);
+  return bf16 ? launch_chunk_of<D, true>(p, fmt, stream) : launch_chunk_of<D, false>(p, fmt, stream);
 }
 
 }  // namespace kv

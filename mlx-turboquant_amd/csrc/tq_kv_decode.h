@@ -442,7 +442,7 @@ __device__ inline void decode_unit(const Params& p, int b, int h, int first, int
     }
     if (orow >= p.rows) continue;
     const float Mr = M == -INFINITY ? 0.f : M, mr = m == -INFINITY ? 0.f : m;
-    const float fin = CACHED ? __builtin_amdgcn_exp2f(Mr - mr) : 1.f;
+    const float fin = (CACHED ? __builtin_amdgcn_exp2f(Mr - mr) : 1.f) / l;
     for (int k = threadIdx.x & 15; k < NP * 16; k += 16) {
       const int i = k % NP, r = k / NP, dim = NO * r + ps * NP + i;  // in the order of the dims
       float x = 0.f;
@@ -451,7 +451,7 @@ __device__ inline void decode_unit(const Params& p, int b, int h, int first, int
       if (slot >= 0) {
         p.ws[p.o_off + ((int64_t)slot * p.rows + orow) * D + dim] = x;
       } else {
-        x = pmin + oi < 0 ? 0.f : x / l * fin;
+        x = pmin + oi < 0 ? 0.f : x * fin;
         const int64_t at = (int64_t)b * p.out.sb + (int64_t)(h * p.group + oh) * p.out.sh + (int64_t)oi * p.out.st + dim;
         if (p.out_f32)
           ((float*)p.out.p)[at] = x;
