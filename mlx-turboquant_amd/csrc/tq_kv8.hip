@@ -1,14 +1,15 @@
 // 8-bit KV cache: quantising keys and values as they are written, and reading
 // them back. Both are bound by memory: 2 bytes in and 1 out per element (and
-// back). One workgroup takes one block of tokens (write) or one 64-token tile
-// (read) of one (row, side).
+// back). One workgroup takes one 64-token tile of one (row, side), whose value
+// codes are 64 whole bytes per dim.
 //
-// Write: the block stays in registers between its maximum and its codes. The
-// maximum is taken on the absolute values' bits, which order 16-bit floats and
-// put infinities and NaN on top. Codes are x * (QMAX / a) in float32, one
-// rounding (v_rndne / v_cvt_pk_fp8, ties to even). Value codes turn in LDS.
-// The workgroup of a sequence's first block also moves the incomplete block:
-// it has read the tail before it writes there.
+// Write: the tile stays in registers between its blocks' maxima and its codes.
+// Maxima are taken on the absolute values' bits, which order 16-bit floats and
+// put infinities and NaN on top; a wave's loads lie in one group of 16 tokens.
+// Codes are x * (QMAX / a) in float32, one rounding (v_rndne / v_cvt_pk_fp8, ties
+// to even). Value codes turn in LDS, 4 x 4 bytes at a time. The workgroup of a
+// call's first tile also moves the incomplete block: it has read the tail before
+// it writes there.
 
 #include "tq_kv8.h"
 
@@ -25,13 +26,23 @@ struct WriteParams {
   int32_t start, n_new, slots, shift;
 };
 
+// Bytes of four dwords, as rows and columns exchanged.
+__device__ inline void turn4(uint32_t (&w)[4]) {
+  const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+  const uint32_t c = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+  w[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+  w[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+  w[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+  w[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+}
+
 template <int D, int BLOCK, bool BF>
 __global__ __launch_bounds__(WT) void write_kernel(const WriteParams p) {
-  constexpr int VEC = BLOCK * D / 8;  // pieces of 8 elements
-  constexpr int PER = (VEC + WT - 1) / WT;
-  constexpr int LP = D + 4;           // LDS row pitch of codes, bytes
-  __shared__ __align__(16) uint8_t lt[BLOCK * LP];
-  __shared__ uint32_t lmax[WT / 64];
+  constexpr int PER = TILE * D / 8 / WT;   // pieces of 8 elements per thread
+  constexpr int PARTS = D / 32;            // maxima of a group of 16 tokens
+  constexpr int LP = D + 4;                // LDS row pitch of codes, bytes
+  __shared__ __align__(16) uint8_t lt[TILE * LP];
+  __shared__ uint32_t part[4][PARTS];
 
   const int side = blockIdx.x & 1;
   const int j = (blockIdx.x >> 1) % p.slots, bh = (blockIdx.x >> 1) / p.slots;
@@ -40,49 +51,61 @@ __global__ __launch_bounds__(WT) void write_kernel(const WriteParams p) {
   const int n = p.n_new_b ? p.n_new_b[b] : p.n_new;
   if (n <= 0 || n > p.n_new || start < 0 || start > p.s.cap - n) return;
   const int end = start + n;
-  const int blk = start / BLOCK + j;
-  const bool full = blk < end / BLOCK;
-  if (!full && j > 0) return;
+  const int t0 = (start / TILE + j) * TILE;
+  const int first = max(t0, start / BLOCK * BLOCK), last = min(t0 + TILE, end / BLOCK * BLOCK);  // of completed blocks
 
   const Rows& src = side ? p.v : p.k;
   const uint16_t* x0 = (const uint16_t*)src.p + (int64_t)b * src.sb + (int64_t)h * src.sh;
   uint16_t* tail = (uint16_t*)(side ? p.s.v_tail : p.s.k_tail) + (int64_t)bh * BLOCK * D;
 
-  if (full) {
-    const int t0 = blk * BLOCK;
+  if (first < last) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     u4 x[PER];
-    uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int vec = i * WT + threadIdx.x, t = vec / (D / 8), c = vec % (D / 8);
+      const int vec = i * WT + threadIdx.x, t = t0 + vec / (D / 8), c = vec % (D / 8);
       x[i] = u4{0, 0, 0, 0};
-      if (vec < VEC) x[i] = t0 + t < start ? *(const u4*)(tail + t * D + c * 8) : *(const u4*)(x0 + (int64_t)(t0 + t - start) * src.st + c * 8);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) top = max(top, max(x[i][k] & 0x7fffu, x[i][k] >> 16 & 0x7fffu));
+      if (t >= first && t < last) x[i] = t < start ? *(const u4*)(tail + t % BLOCK * D + c * 8) : *(const u4*)(x0 + (int64_t)(t - start) * src.st + c * 8);
     }
 #pragma unroll
-    for (int k = 1; k < 64; k *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, k));
-    if ((threadIdx.x & 63) == 0) lmax[threadIdx.x >> 6] = top;
-    __syncthreads();
+    for (int i = 0; i < PER; ++i) {
+      uint32_t top = 0;
 #pragma unroll
-    for (int k = 0; k < WT / 64; ++k) top = max(top, lmax[k]);
-    const float a = elem<BF>(top);
+      for (int k = 0; k < 4; ++k) top = top16(top, x[i][k]);
+      top = max(top & 0xffffu, top >> 16);
+#pragma unroll
+      for (int k = 1; k < 64; k *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, k));
+      const int w = i * (WT / 64) + wave;  // 64 pieces; 2 D of them are 16 tokens
+      if (lane == 0) part[w / PARTS][w % PARTS] = top;
+    }
+    __syncthreads();
     const float qmax = p.s.fmt == TQ_KV8_INT8 ? QMAX_INT8 : QMAX_E4M3;
-    const bool finite = top < (BF ? 0x7f80u : 0x7c00u), codes = finite && a >= TINY;
-    const float inv = codes ? qmax / a : 0.f;
-    if (threadIdx.x == 0) (side ? p.s.v_scales : p.s.k_scales)[(int64_t)bh * (p.s.cap >> p.shift) + blk] = codes ? a / qmax : finite ? 0.f : NAN;
+    float inv[TILE / BLOCK];
+#pragma unroll
+    for (int g = 0; g < TILE / BLOCK; ++g) {
+      uint32_t top = 0;
+      for (int k = 0; k < BLOCK / 16 * PARTS; ++k) top = max(top, part[g * (BLOCK / 16) + k / PARTS][k % PARTS]);
+      const float a = elem<BF>(top);
+      const bool finite = top < (BF ? 0x7f80u : 0x7c00u), codes = finite && a >= TINY;
+      inv[g] = codes ? qmax / a : 0.f;
+      const int t = t0 + g * BLOCK;
+      if (threadIdx.x == 0 && t >= first && t < last)
+        (side ? p.s.v_scales : p.s.k_scales)[(int64_t)bh * (p.s.cap >> p.shift) + t / BLOCK] = codes ? a / qmax : finite ? 0.f : NAN;
+    }
 
     uint8_t* kc = p.s.k_codes + ((int64_t)bh * p.s.cap + t0) * D;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int vec = i * WT + threadIdx.x;
-      if (vec >= VEC) break;
+      const int vec = i * WT + threadIdx.x, t = vec / (D / 8), c = vec % (D / 8);
+      float f = inv[0];
+#pragma unroll
+      for (int g = 1; g < TILE / BLOCK; ++g) f = t / BLOCK == g ? inv[g] : f;
       u2 w = {0, 0};
-      if (codes) {
+      if (f > 0.f) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float c0 = elem<BF>(x[i][2 * k] & 0xffff) * inv, c1 = elem<BF>(x[i][2 * k] >> 16) * inv;
-          const float c2 = elem<BF>(x[i][2 * k + 1] & 0xffff) * inv, c3 = elem<BF>(x[i][2 * k + 1] >> 16) * inv;
+          const float c0 = elem<BF>(x[i][2 * k] & 0xffff) * f, c1 = elem<BF>(x[i][2 * k] >> 16) * f;
+          const float c2 = elem<BF>(x[i][2 * k + 1] & 0xffff) * f, c3 = elem<BF>(x[i][2 * k + 1] >> 16) * f;
           if (p.s.fmt == TQ_KV8_INT8) {
             w[k] = ((uint32_t)(int)rintf(c0) & 0xff) | ((uint32_t)(int)rintf(c1) & 0xff) << 8 | ((uint32_t)(int)rintf(c2) & 0xff) << 16 |
                    (uint32_t)(int)rintf(c3) << 24;
@@ -93,34 +116,35 @@ __global__ __launch_bounds__(WT) void write_kernel(const WriteParams p) {
         }
       }
       if (side == 0) {
-        *(u2*)(kc + vec * 8) = w;
+        if (t0 + t >= first && t0 + t < last) *(u2*)(kc + vec * 8) = w;
       } else {
-        const int t = vec / (D / 8), c = vec % (D / 8);
         *(uint32_t*)(lt + t * LP + c * 8) = w.x;
         *(uint32_t*)(lt + t * LP + c * 8 + 4) = w.y;
       }
     }
     if (side == 1) {
       __syncthreads();
-      uint8_t* vc = p.s.v_codes + ((int64_t)bh * p.s.cap + (t0 / TILE) * TILE) * D + t0 % TILE;
-      for (int i = threadIdx.x; i < D * BLOCK / 16; i += WT) {
-        const int dim = i / (BLOCK / 16), c = i % (BLOCK / 16);
-        u4 w;
+      uint8_t* vc = p.s.v_codes + ((int64_t)bh * p.s.cap + t0) * D;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint8_t* q = lt + (c * 16 + 4 * k) * LP + dim;
-          w[k] = (uint32_t)q[0] | (uint32_t)q[LP] << 8 | (uint32_t)q[2 * LP] << 16 | (uint32_t)q[3 * LP] << 24;
-        }
-        *(u4*)(vc + (int64_t)dim * TILE + c * 16) = w;
+      for (int i = threadIdx.x; i < D / 4 * (TILE / 8); i += WT) {  // 4 dims x 8 tokens
+        const int c = i % (TILE / 8), dim = i / (TILE / 8) * 4, t = t0 + c * 8;
+        if (t < first || t >= last) continue;
+        uint32_t w[2][4];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k / 4][k % 4] = *(const uint32_t*)(lt + (c * 8 + k) * LP + dim);
+        turn4(w[0]);
+        turn4(w[1]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) *(u2*)(vc + (dim + k) * TILE + c * 8) = u2{w[0][k], w[1][k]};
       }
     }
   }
 
   if (j == 0) {  // the incomplete block's tokens (what the tail held has been read)
     __syncthreads();
-    const int t0 = max(start, end / BLOCK * BLOCK);
-    for (int i = threadIdx.x; i < (end - t0) * (D / 8); i += WT) {
-      const int t = t0 + i / (D / 8), c = i % (D / 8);
+    const int at = max(start, end / BLOCK * BLOCK);
+    for (int i = threadIdx.x; i < (end - at) * (D / 8); i += WT) {
+      const int t = at + i / (D / 8), c = i % (D / 8);
       *(u4*)(tail + t % BLOCK * D + c * 8) = *(const u4*)(x0 + (int64_t)(t - start) * src.st + c * 8);
     }
   }
@@ -282,7 +306,8 @@ extern "C" int tq_kv8_write(const tq_kv8_store* store, const tq_rows4* k, const 
   p.n_new_b = n_new_b;
   p.start = start;
   p.n_new = n_new;
-  p.slots = (n_new + store->block - 1) / store->block;
+  p.slots = (n_new + kv::TILE - 2) / kv::TILE + 1;  // tiles that n_new tokens touch at most, wherever they start
+  if (start_b == nullptr) p.slots = (start + n_new - 1) / kv::TILE - start / kv::TILE + 1;
   p.shift = store->block == 16 ? 4 : store->block == 32 ? 5 : 6;
   const int64_t wgs = (int64_t)store->batch * store->heads * p.slots * 2;
   if (wgs >= (int64_t)1 << 31) return set_error(TQ_ERR_UNSUPPORTED, "kv8 write: too many blocks in one call");

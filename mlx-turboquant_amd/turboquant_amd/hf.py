@@ -15,7 +15,8 @@ model the same roles are:
   SDPA mask construction): for a one-token decode step it runs the fused
   decode-attention kernel over the packed codes (``TurboQuantKVCache.attend``,
   never materialising the dense K/V) or the dense decode kernel over an
-  ``FP16KVCache`` (fp16 / bf16, head_dim 128); every other call (prefill, the
+  ``FP16KVCache`` (fp16 / bf16, head_dim 128) or the 8-bit kernels over a
+  ``KV8Cache`` (a ``sliding_window`` included); every other call (prefill, the
   model's default layers) is ``transformers``' SDPA over the dense K/V, as in
   the reference. The kernels take no mask, logit soft-capping, sliding window
   or attention sinks: a decode step that carries any of them (a padding mask,
@@ -47,6 +48,7 @@ from transformers.integrations.sdpa_attention import sdpa_attention_forward
 from transformers.masking_utils import AttentionMaskInterface, sdpa_mask
 
 from .cache import ATTEND_GROUPS, TurboQuantKVCache
+from .kv8 import HEAD_DIMS as KV8_HEAD_DIMS, KV8Cache
 from .patch import FP16KVCache
 
 ATTN_IMPLEMENTATION = "turboquant"
@@ -66,17 +68,19 @@ def fused_supported(cache, hq: int, hkv: int, head_dim: int) -> bool:
     """Whether the decode kernels serve a layer of this shape: the packed
     route (``TurboQuantKVCache.attend``: any integer query-head ratio) or the
     dense fp16 / bf16 kernel (``FP16KVCache.attend``: head_dim 128, ratios
-    1, 2, 4, 8)."""
+    1, 2, 4, 8) or the 8-bit one (``KV8Cache.attend``: any ratio)."""
     if hkv <= 0 or hq % hkv:
         return False
     if isinstance(cache, FP16KVCache):
         return head_dim == 128 and hq // hkv in ATTEND_GROUPS
+    if isinstance(cache, KV8Cache):
+        return head_dim in KV8_HEAD_DIMS
     return TurboQuantKVCache.attend_head_dim(head_dim)
 
 
 class TurboQuantLayer(CacheLayerMixin):
-    """One attention layer over a ``TurboQuantKVCache`` (compressed) or an
-    ``FP16KVCache`` (uncompressed). ``update`` appends the new tokens
+    """One attention layer over a ``TurboQuantKVCache`` (compressed), an
+    ``FP16KVCache`` (uncompressed) or a ``KV8Cache`` (8 bits). ``update`` appends the new tokens
     (draining the oldest residual tokens into the packed store) and returns
     the dense K/V in the input dtype, or, for a one-token step with ``fused``,
     the new tokens themselves tagged for the decode kernel."""
@@ -96,6 +100,8 @@ class TurboQuantLayer(CacheLayerMixin):
         if isinstance(self.cache, FP16KVCache):  # the dense kernel's shapes
             self.fused = self.fused and key_states.is_cuda and key_states.shape[-1] == 128 and \
                 key_states.dtype in (torch.float16, torch.bfloat16)
+        elif isinstance(self.cache, KV8Cache) and key_states.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"an 8-bit layer takes fp16 or bf16 keys and values, got {key_states.dtype}")
         self.is_initialized = True
 
     def fused_step(self, key_states) -> bool:
@@ -157,7 +163,7 @@ class TurboQuantCache(Cache):
         hq, hkv, hd = model_heads(model.config)
         layers = []
         for i, c in enumerate(caches):
-            if isinstance(c, (TurboQuantKVCache, FP16KVCache)):
+            if isinstance(c, (TurboQuantKVCache, FP16KVCache, KV8Cache)):
                 layers.append(TurboQuantLayer(c, fused and fused_supported(c, hq, hkv, hd), model.config))
             else:
                 layers.append(defaults[i] if i < len(defaults) else DynamicLayer())
@@ -215,6 +221,12 @@ def turboquant_attention(module, query, key, value, attention_mask, dropout: flo
     window = kwargs.get("sliding_window")
     if layer is not None:
         tk = layer.get_seq_length()
+        if attention_mask is None and not softcap and sinks is None and isinstance(layer.cache, KV8Cache):
+            # the 8-bit kernels take a window; straight to the layout returned
+            B, hq, T, D = query.shape
+            out = torch.empty(B, T, hq, D, dtype=query.dtype, device=query.device)
+            layer.cache.attend(query, scale=scaling, out=out.transpose(1, 2), window=window or None)
+            return out, None
         if attention_mask is None and not softcap and sinks is None and not (window and tk > window):
             out = layer.cache.attend(query, scale=scaling)  # (B, Hq, 1, D) float32
             return out.to(query.dtype).transpose(1, 2).contiguous(), None

@@ -34,6 +34,7 @@ import numpy as np
 import torch
 
 from .cache import TurboQuantKVCache
+from .kv8 import HEAD_DIMS as KV8_HEAD_DIMS, KV8Cache
 
 
 class FP16KVCache:
@@ -41,7 +42,7 @@ class FP16KVCache:
     hands those layers mlx-lm's ``KVCache``, patch.py:337-338). Storage grows
     in steps of ``step`` tokens, as mlx-lm's KVCache does; ``keys`` /
     ``values`` are views of the first ``offset`` tokens. ``attend`` runs the
-    dense decode-attention kernel over them (fp16 / bf16, head_dim 128)."""
+    attention kernels over them (fp16 / bf16)."""
 
     step = 256
 
@@ -77,13 +78,24 @@ class FP16KVCache:
         self.update(keys, values)
         return self.keys, self.values
 
-    def attend(self, queries, scale=None, out=None):
-        """Decode attention of one query token per head over the cached tokens:
-        float32 (B, Hq, 1, D)."""
+    def attend(self, queries, scale=None, out=None, window=None, sinks=0):
+        """Attention of the cache's last T_q tokens over it: float32
+        (B, Hq, T_q, D). One query token and no ``window``: the dense decode
+        kernel (head_dim 128). Several (causal), or with a ``window`` (each sees
+        the last ``window`` tokens up to its own and the first ``sinks``):
+        ``window_attention``, head dims 64, 96, 128 and 256."""
         if self._k is None or self.offset == 0:
             raise ValueError("attend() on an empty cache")
-        from .cache import dense_attention
-        return dense_attention(queries, self.keys, self.values, scale=scale, out=out)
+        q = queries if queries.dim() == 4 else queries[:, :, None]
+        if window is None and q.shape[2] == 1:
+            from .cache import dense_attention
+            return dense_attention(queries, self.keys, self.values, scale=scale, out=out)
+        if q.shape[2] > self.offset:
+            raise ValueError(f"{q.shape[2]} query tokens > the {self.offset} cached tokens")
+        from .window import window_attention
+        if out is None:
+            out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+        return window_attention(q, self.keys, self.values, window, sinks, scale=scale, out=out)
 
     def make_mask(self, N, offset=0, return_array=False, window_size=None):
         return None if N == 1 and not return_array else "causal"
@@ -276,8 +288,14 @@ def apply_turboquant(model, key_bits: float = 4, value_bits: float = 2, residual
                      num_layers: int | None = None, rotation_seed: int = 42,
                      skip_layers: list[int] | None = None, auto_detect_outliers: bool = True,
                      fp16_sink_size: int = 0, chunk_size: int = 0, qjl_correction: bool = False,
-                     qjl_n_proj: int = 32):
-    """Install TurboQuant caches on ``model`` (patch.py:136-371)."""
+                     qjl_n_proj: int = 32, skip_layer_format: str = "fp16"):
+    """Install TurboQuant caches on ``model`` (patch.py:136-371).
+
+    ``skip_layer_format``: what the outlier / skipped layers are held in:
+    ``"fp16"`` (uncompressed, as in the reference), or ``"int8"`` / ``"fp8"``:
+    a ``KV8Cache``, half the bytes."""
+    if skip_layer_format not in ("fp16", "int8", "fp8"):
+        raise ValueError(f"skip_layer_format {skip_layer_format!r}: use 'fp16', 'int8' or 'fp8'")
     if head_dim is None or num_kv_heads is None or num_layers is None:
         config = _get_model_config(model)
     else:
@@ -285,6 +303,9 @@ def apply_turboquant(model, key_bits: float = 4, value_bits: float = 2, residual
     hd = head_dim or config["head_dim"]
     nkv = num_kv_heads or config["num_kv_heads"]
     nl = num_layers or config["num_layers"]
+
+    if skip_layer_format != "fp16" and hd not in KV8_HEAD_DIMS:
+        raise ValueError(f"skip_layer_format {skip_layer_format!r}: head_dim {hd} is not one of {KV8_HEAD_DIMS}")
 
     # few KV heads -> more precision (patch.py:198-217)
     if nkv <= 2 and key_bits < 4:
@@ -338,7 +359,8 @@ def apply_turboquant(model, key_bits: float = 4, value_bits: float = 2, residual
             if i in default_layers:
                 caches.append(defaults[i] if i < len(defaults) else None)
             elif i in layers_to_skip:
-                caches.append(FP16KVCache())
+                caches.append(FP16KVCache() if skip_layer_format == "fp16" else
+                              KV8Cache(head_dim=hd, num_kv_heads=nkv, fmt=skip_layer_format))
             else:
                 caches.append(TurboQuantKVCache(
                     head_dim=hd, num_kv_heads=nkv, key_bits=key_bits, value_bits=value_bits,
@@ -353,6 +375,7 @@ def apply_turboquant(model, key_bits: float = 4, value_bits: float = 2, residual
         "value_bits": value_bits, "residual_window": residual_window, "fp16_sink_size": fp16_sink_size,
         "chunk_size": chunk_size, "qjl_correction": qjl_correction, "qjl_n_proj": qjl_n_proj,
         "skip_layers": sorted(layers_to_skip), "default_cache_layers": sorted(default_layers),
+        "skip_layer_format": skip_layer_format,
     }
     return model
 

@@ -259,3 +259,32 @@ def test_workspace_is_bounded_by_what_a_window_reads():
 
     assert need(window=1024, sinks=4) < need() and need(window=1024, max_len=2000) <= need(window=1024)
     assert need(window=1 << 20) == need() and math.isfinite(need(batch=1000))
+
+
+def _model(head_dim=128, layers=4):
+    import types
+    return types.SimpleNamespace(config=types.SimpleNamespace(
+        num_hidden_layers=layers, num_key_value_heads=8, num_attention_heads=8, hidden_size=8 * head_dim, head_dim=head_dim))
+
+
+def test_skipped_layers_in_8_bits():
+    from turboquant_amd import TurboQuantKVCache, apply_turboquant
+    from turboquant_amd.patch import FP16KVCache
+    for fmt in ("int8", "fp8"):
+        m = apply_turboquant(_model(), skip_layers=[1, 3], auto_detect_outliers=False, skip_layer_format=fmt)
+        assert [type(c) for c in m.make_cache()] == [TurboQuantKVCache, KV8Cache, TurboQuantKVCache, KV8Cache]
+        assert m.make_cache()[1].fmt == fmt and m._turboquant_config["skip_layer_format"] == fmt
+    m = apply_turboquant(_model(), skip_layers=[1], auto_detect_outliers=False)
+    assert type(m.make_cache()[1]) is FP16KVCache
+    with pytest.raises(ValueError, match="skip_layer_format"):
+        apply_turboquant(_model(), skip_layer_format="int4")
+    with pytest.raises(ValueError, match="head_dim 80"):
+        apply_turboquant(_model(80), skip_layer_format="int8")
+
+
+def test_8_bit_layer_in_transformers_refuses_float32():
+    pytest.importorskip("transformers")
+    from turboquant_amd.hf import TurboQuantLayer, fused_supported
+    with pytest.raises(ValueError, match="fp16 or bf16"):
+        TurboQuantLayer(KV8Cache(64, 2)).update(x(1, 2, 3, 64).float(), x(1, 2, 3, 64).float())
+    assert fused_supported(KV8Cache(96, 2), 6, 2, 96) and not fused_supported(KV8Cache(64, 2), 3, 2, 64)
