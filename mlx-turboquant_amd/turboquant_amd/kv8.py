@@ -128,13 +128,16 @@ class KV8Store:
         code, dev, dtype = FORMATS[fmt][1], k_codes.device, k_tail.dtype
         if cap % TILE:
             raise ValueError(f"k_codes: room for {cap} tokens, not a multiple of {TILE}")
+        tensors = (k_codes, v_codes, k_scales, v_scales, k_tail, v_tail)
         scales, tail = (B, H, cap // block), (B, H, block, D)
-        for t, shape, kind in ((k_codes, k_codes.shape, code), (v_codes, (B, H, cap // TILE, D, TILE), code),
-                               (k_scales, scales, torch.float32), (v_scales, scales, torch.float32),
-                               (k_tail, tail, dtype), (v_tail, tail, dtype)):
-            if t.shape != shape or t.dtype != kind or t.device != dev or not t.is_contiguous():
-                raise ValueError(f"store: expected a contiguous {kind} tensor of shape {tuple(shape)} on {dev}, got "
-                                 f"{t.dtype} {tuple(t.shape)} on {t.device}")
+        shapes = [(B, H, cap, D), (B, H, cap // TILE, D, TILE), scales, scales, tail, tail]
+        kinds = [code, code, torch.float32, torch.float32, dtype, dtype]
+        if ([t.shape for t in tensors] != shapes or [t.dtype for t in tensors] != kinds or
+                not all([t.is_contiguous() for t in tensors]) or any([t.device != dev for t in tensors])):
+            for name, t, shape, kind in zip(("k_codes", "v_codes", "k_scales", "v_scales", "k_tail", "v_tail"), tensors, shapes, kinds):
+                if t.shape != shape or t.dtype != kind or t.device != dev or not t.is_contiguous():
+                    raise ValueError(f"{name}: expected a contiguous {kind} tensor of shape {shape} on {dev}, got "
+                                     f"{t.dtype} {tuple(t.shape)} on {t.device}")
         self.fmt, self.block, self.batch, self.heads, self.cap, self.head_dim = fmt, block, B, H, cap, D
         self.dtype, self.device = dtype, dev
         self.k_codes, self.v_codes, self.k_scales, self.v_scales = k_codes, v_codes, k_scales, v_scales
@@ -267,7 +270,7 @@ def _attention_desc(queries, B, hkv, D, dtype, device, len_b, max_len, scale, wi
         raise ValueError(f"sinks {sinks}")
     code = out_code = _lib.dtype_code(dtype)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(shape, dtype=dtype, device=device)
         o = (out.data_ptr(), *out.stride()[:3])
     else:
         if out.shape != shape or out.dtype not in (dtype, torch.float32) or out.device != device:
