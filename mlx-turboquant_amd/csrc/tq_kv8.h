@@ -103,11 +103,11 @@ __device__ inline uint32_t bits2(float a, float b) {
     return __builtin_bit_cast(uint32_t, h2{(_Float16)a, (_Float16)b});
 }
 
-// Values that are infinite or NaN, in tiles that some rows see only in part:
-// taken out of the product (0 x inf would reach the rows that do not see them)
-// and counted in one of their own, marks x seen: 1 for inf, 128 for -inf, 2^14
-// for NaN (at most 64 of each per tile: exact), which gives back what the rows
-// that see them get.
+// Values that are infinite or NaN: taken out of the product (0 x inf would reach
+// rows that do not see them, and the remainders of split weights are 0) and
+// counted in one of their own, marks x seen: 1 for inf, 128 for -inf, 2^14 for
+// NaN (at most 64 of each per tile: exact), which gives what the rows that see
+// them get.
 // The larger of two pairs of 16-bit magnitudes (signs off), half by half; whether
 // either is that of an infinity or NaN.
 __device__ inline uint32_t top16(uint32_t a, uint32_t x) {

@@ -25,7 +25,7 @@
 // two bf16 parts.
 //
 // Masked scores are -inf and their weights 0; infinite and NaN values in 16-bit
-// tiles that some rows see only in part are taken apart (marks()).
+// tiles are taken apart (marks()).
 #pragma once
 
 #include <math.h>
@@ -48,7 +48,7 @@ struct Decode {
   int n, g;           // query row (column of S^T), lane group
   int pos, low;       // the row sees tokens t <= pos with t > low or t < sinks
   int pmin, pmax, lowmax;
-  float cn;           // scale * log2 e (times the power of two taken off q)
+  float cn, cx;       // scale * log2 e, times the power of two taken off q in two parts
   u4 q[NS];
   f4 o[NO];
   float M, m, l;
@@ -67,7 +67,7 @@ struct Decode {
   }
 
   // bf16 rows to fp16: times 2^e, the row's largest element to [2^14, 2^15)
-  __device__ float to_f16(u4 (&f)[NS]) const {
+  __device__ void to_f16(u4 (&f)[NS]) {
     float top = 0.f;
 #pragma unroll
     for (int st = 0; st < NS; ++st)
@@ -84,7 +84,9 @@ struct Decode {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         f[st][i] = bits2<false>(ldexpf(elem<true>(f[st][i] & 0xffff), e), ldexpf(elem<true>(f[st][i] >> 16), e));
-    return ldexpf(1.f, -e);
+    // both normal numbers; a key scale comes between them
+    cn *= ldexpf(1.f, -e / 2);
+    cx = ldexpf(1.f, -(e - e / 2));
   }
 
   // Scores (masked: -inf) to weights, and the running maxima and sum.
@@ -166,7 +168,7 @@ struct Decode {
     const int t0 = tile * TILE;
     if (!AHEAD) load_k(kc, ksc, tile);
     float s[16], w[16];
-    const float cs = cn * ks;
+    const float cs = BF ? cn * ks * cx : cn * ks;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       f4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -284,12 +286,10 @@ struct Decode {
       if constexpr (BF) px[i] = bits2<true>(w[2 * i] - elem<true>(pw[i] & 0xffff), w[2 * i + 1] - elem<true>(pw[i] >> 16));
     }
     uint32_t top = 0;
-    if (masked) {
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
+    for (int u = 0; u < 8; ++u)
 #pragma unroll
-        for (int i = 0; i < NO / 2; ++i) top = top16(top, v16[u][i]);
-    }
+      for (int i = 0; i < NO / 2; ++i) top = top16(top, v16[u][i]);
     const bool apart = __any(odd16<BF>(top));
     const u4 ones = {seen2<BF>(seen), seen2<BF>(seen >> 2), seen2<BF>(seen >> 4), seen2<BF>(seen >> 6)};
 #pragma unroll
@@ -359,7 +359,7 @@ __device__ inline void decode_unit(const Params& p, int b, int h, int first, int
       w.load_v(vc, vsc, tl.at(i));
     }
     w.load_q(qp, live, w.q);
-    if constexpr (BF) w.cn *= w.to_f16(w.q);
+    if constexpr (BF) w.to_f16(w.q);
     for (; i < end; i += DEC_WAVES)
       w.tile8(kc, vc, ksc, vsc, tl.at(i), i + DEC_WAVES < end ? tl.at(i + DEC_WAVES) : -1, tl.main_len);
     if (i < last) {  // the tail

@@ -79,6 +79,16 @@ def _rows4(t: torch.Tensor) -> tuple[tuple[int, int, int, int], torch.Tensor]:
     return (p, sb, sh, st), t
 
 
+def _overlaps(t: torch.Tensor) -> bool:
+    """Whether elements of ``t`` may share memory (dims that do not nest)."""
+    span = 1
+    for stride, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
+        if stride < span:
+            return True
+        span = stride * n
+    return False
+
+
 def _lengths(lens, batch: int, cap: int, device, what: str) -> tuple[int, int]:
     """(device array or 0, the length where there is one for all)."""
     if isinstance(lens, torch.Tensor):
@@ -103,8 +113,8 @@ class KV8Store:
     def __init__(self, batch: int, heads: int, head_dim: int, capacity: int, fmt: str = "int8", block: int = 32,
                  dtype: torch.dtype = torch.bfloat16, device=None):
         dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
-        if capacity < 0:
-            raise ValueError(f"capacity {capacity}")
+        if batch < 0 or heads < 1 or capacity < 0:
+            raise ValueError(f"batch {batch}, heads {heads}, capacity {capacity}")
         _check(fmt, head_dim, block, dtype)
         cap = (capacity + TILE - 1) // TILE * TILE
         code = FORMATS[fmt][1]
@@ -124,6 +134,8 @@ class KV8Store:
 
     def _set(self, fmt, k_codes, v_codes, k_scales, v_scales, k_tail, v_tail) -> None:
         B, H, cap, D = k_codes.shape
+        if H == 0:
+            raise ValueError("no kv heads")
         block = k_tail.shape[2]
         code, dev, dtype = FORMATS[fmt][1], k_codes.device, k_tail.dtype
         if cap % TILE:
@@ -276,8 +288,8 @@ def _attention_desc(queries, B, hkv, D, dtype, device, len_b, max_len, scale, wi
         if out.shape != shape or out.dtype not in (dtype, torch.float32) or out.device != device:
             raise ValueError(f"out: expected {tuple(shape)} of {dtype} or float32 on {device}")
         o, same = _rows4(out)
-        if same is not out:
-            raise ValueError("out: rows must be contiguous and 16-byte aligned, strides multiples of 8")
+        if same is not out or _overlaps(out):
+            raise ValueError("out: rows must be contiguous, 16-byte aligned and apart, strides multiples of 8")
         out_code = _lib.dtype_code(out.dtype)
     rows, q = _rows4(q)
     desc = _DESC.pack(B, shape[1], hkv, D, shape[2], code, out_code, 0 if window is None else min(window, _MOST),

@@ -407,6 +407,85 @@ def test_bf16_queries_of_any_size():
         check(kv8_attention(q, store, T)[0], want, tol, torch.bfloat16)
 
 
+@pytest.mark.parametrize("e", [-128, 112])
+def test_bf16_queries_at_the_ends_of_their_range(e):
+    """Queries down to subnormal numbers, and up, with keys that bring the scores back to a few units."""
+    from turboquant_amd import kv8_attention
+    D, T = 64, 70
+    k = (rand(120, 1, 1, T, D).float() * 2.0 ** min(-e, 124)).bfloat16()
+    q = (rand(121, 1, 2, 1, D).float() * 2.0 ** e).bfloat16()
+    v = rand(122, 1, 1, T, D, dtype=torch.bfloat16)
+    store = store_of(k, "fp8", 32, T, v)
+    want, tol = attend(q[0], exact_tokens(k[0], T, "fp8", 32), exact_tokens(v[0], T, "fp8", 32), T, 0, 0, weights=torch.float16)
+    check(kv8_attention(q, store, T)[0], want, tol, torch.bfloat16)
+
+
+@pytest.mark.parametrize("B", [65, 200])
+def test_many_sequences(B):
+    """More sequences than a wave has lanes, empty ones among them, over enough tiles that they are shared out."""
+    from turboquant_amd import kv8_attention, window_attention
+    D, hq, H, cap = 64, 2, 1, 4096
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, cap + 1, (B,), generator=g)
+    lens[[0, 3, 63, 64, B - 1]] = torch.tensor([0, 0, 5, 4096, 0])
+    lens[10:60] = 0
+    k, v, q = rand(123, B, H, cap, D), rand(124, B, H, cap, D), rand(125, B, hq, 1, D)
+    store = store_of(k, "int8", 64, cap, v)
+    for b, n in enumerate(lens.tolist()):
+        full = n // 64 * 64
+        store.k_tail[b, :, :n - full], store.v_tail[b, :, :n - full] = k[b, :, full:n], v[b, :, full:n]
+    lt = lens.to(torch.int32).to(DEV)
+    got, dense = kv8_attention(q, store, lt), window_attention(q, k, v, lens=lt)
+    windowed = window_attention(q, k, v, 3000, 70, lens=lt)
+    for b in sorted({0, 1, 3, 9, 60, 62, 63, 64, B // 2, B - 2, B - 1}):
+        n = int(lens[b])
+        if n == 0:
+            assert (got[b] == 0).all() and (dense[b] == 0).all() and (windowed[b] == 0).all()
+            continue
+        want, tol = attend(q[b], exact_tokens(k[b], n, "int8", 64), exact_tokens(v[b], n, "int8", 64), n, 0, 0, weights=torch.float16)
+        check(got[b], want, tol, q.dtype, f"8-bit, {b}")
+        want, tol = attend(q[b], k[b, :, :n], v[b, :, :n], n, 0, 0, weights=torch.float16)
+        check(dense[b], want, tol, q.dtype, f"16-bit, {b}")
+        want, tol = attend(q[b], k[b, :, :n], v[b, :, :n], n, 3000, 70, weights=torch.float16)
+        check(windowed[b], want, tol, q.dtype, f"windowed, {b}")
+
+
+@pytest.mark.parametrize("nq", [1, 40])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_infinite_values_that_are_seen(nq, dtype):
+    """+inf gives +inf, -inf gives -inf, both or NaN give NaN, in tiles that all rows see and in those that some do."""
+    from turboquant_amd import window_attention
+    D, T = 64, 300
+    k, v, q = rand(126, 1, 1, T, D, dtype=dtype, scale=0.2), rand(127, 1, 1, T, D, dtype=dtype), rand(128, 1, 2, nq, D, dtype=dtype)
+    v[0, 0, 10, 0] = v[0, 0, T - 1, 1] = math.inf
+    v[0, 0, 70, 2] = v[0, 0, T - 1, 3] = -math.inf
+    v[0, 0, 5, 4], v[0, 0, 200, 4], v[0, 0, 6, 5] = math.inf, -math.inf, math.nan
+    got = window_attention(q, k, v).float().cpu()
+    assert (got[..., 0] == math.inf).all() and (got[..., 2] == -math.inf).all() and torch.isnan(got[..., 4:6]).all()
+    assert (got[:, :, -1, 1] == math.inf).all() and (got[:, :, -1, 3] == -math.inf).all()
+    assert torch.isfinite(got[:, :, :-1, [1, 3]]).all() and torch.isfinite(got[..., 6:]).all()
+
+
+def test_captured_chunk_replays():
+    """A chunk's attention in a HIP graph (more LDS than a launch has by default), split and not, replayed with eager work between."""
+    from turboquant_amd import kv8_attention, window_attention
+    for D, T, nq in ((128, 3000, 60), (256, 500, 200)):
+        k, v, q = rand(129, 1, 2, T, D), rand(130, 1, 2, T, D), rand(131, 1, 4, nq, D)
+        store, lens = store_of(k, "fp8", 32, T, v), torch.full((1,), T, dtype=torch.int32, device=DEV)
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            a, b = kv8_attention(q, store, lens), window_attention(q, k, v, 100, 4, lens=lens)
+        for i in range(4):
+            q.copy_(rand(140 + i, 1, 4, nq, D))
+            n = T - 37 * i // 32 * 32  # whole blocks: the tail of another length is not there
+            n = n // 32 * 32 if i else T
+            lens.fill_(n)
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(a, kv8_attention(q, store, lens)) and torch.equal(b, window_attention(q, k, v, 100, 4, lens=lens)), (D, i)
+
+
 def test_offsets_past_31_bits():
     """Tokens whose codes lie past 2^31 bytes: written, read back and attended to in place."""
     from turboquant_amd import KV8Store, kv8_attention, kv8_read, kv8_write, window_attention

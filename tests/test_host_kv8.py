@@ -118,6 +118,9 @@ def x(*shape, dtype=H16):
     (lambda s: kv8_attention(x(2, 4, 1, 64), s, 10, out=x(2, 4, 2, 64)), "out"),
     (lambda s: kv8_attention(x(2, 4, 1, 64), s, 10, out=x(2, 4, 1, 64, dtype=torch.bfloat16)), "out"),
     (lambda s: kv8_attention(x(2, 4, 3, 64), s, 10, out=x(2, 4, 64, 3).transpose(2, 3)), "out"),
+    (lambda s: kv8_attention(x(2, 4, 3, 64), s, 10, out=x(2, 4, 1, 64).expand(2, 4, 3, 64)), "out"),
+    (lambda s: kv8_attention(x(2, 4, 3, 64), s, 10, out=x(2000).as_strided((2, 4, 3, 64), (256, 64, 32, 1))), "out"),
+    (lambda s: KV8Store(1, 0, 64, 64, device="cpu"), "heads 0"),
     (lambda s: window_attention(x(2, 4, 1, 64), x(2, 2, 9, 64), x(2, 2, 8, 64)), "keys and values"),
     (lambda s: window_attention(x(2, 4, 1, 80), x(2, 2, 9, 80), x(2, 2, 9, 80)), "head_dim 80"),
     (lambda s: window_attention(x(2, 4, 1, 64).float(), x(2, 2, 9, 64).float(), x(2, 2, 9, 64).float()), "fp16 or bf16"),
