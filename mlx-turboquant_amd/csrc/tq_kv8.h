@@ -148,6 +148,11 @@ __device__ inline uint32_t seen_bits(int t, int count, int end, int pos, int low
   const auto below = [&](int x) { return (1u << min(max(x - t, 0), count)) - 1u; };  // tokens before x
   return below(min(end, pos + 1)) & (~below(low + 1) | below(sinks));
 }
+// x where bit k is set, else -inf (a bit field and a merge).
+__device__ inline float seen_or(uint32_t bits, int k, float x) {
+  const uint32_t m = __builtin_amdgcn_sbfe(bits, k, 1);
+  return __uint_as_float((__float_as_uint(x) & m) | (0xff800000u & ~m));
+}
 // 1.0 in the halves whose token is seen (bits 0 and 1)
 template <bool BF>
 __device__ inline uint32_t seen2(uint32_t bits) {

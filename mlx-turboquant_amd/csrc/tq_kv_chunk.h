@@ -301,12 +301,15 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(cons
       for (int g = 0; g < 4; ++g) {
         const uint32_t seen = seen_bits(t0 + 16 * g + 8 * hf, 8, t0 + nv, pos, low, p.sinks);
         // a block without a finite scale: NaN where it is seen only
-        const float bad = x.sc[g] + x.lf[g], nan = bad == bad ? 0.f : bad;
-        if (bad != bad) x.sc[g] = scale, x.lf[g] = 0.f;
+        float nan = 0.f;
+        if constexpr (CACHED) {
+          const float bad = x.sc[g] + x.lf[g];
+          if (bad != bad) nan = bad, x.sc[g] = scale, x.lf[g] = 0.f;
+        }
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float y = s[g >> 1][(g & 1) * 8 + k] + nan;
-          s[g >> 1][(g & 1) * 8 + k] = seen >> k & 1 ? y : -INFINITY;
+          const float y = s[g >> 1][(g & 1) * 8 + k];
+          s[g >> 1][(g & 1) * 8 + k] = seen_or(seen, k, CACHED ? y + nan : y);
         }
       }
     }

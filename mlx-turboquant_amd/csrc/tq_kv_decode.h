@@ -196,7 +196,7 @@ struct Decode {
     if (masked) {
       const uint32_t seen = seen_bits(t0 + 16 * g, 16, main_len, pos, low, p.sinks);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = seen >> i & 1 ? s[i] : -INFINITY;
+      for (int i = 0; i < 16; ++i) s[i] = seen_or(seen, i, s[i]);
       if (t0 + 16 * g >= main_len) {  // not written yet: any bytes
 #pragma unroll
         for (int i = 0; i < NO; ++i) vr[i] = u4{0, 0, 0, 0};
@@ -276,7 +276,7 @@ struct Decode {
     if (masked) {
       seen = seen_bits(t0 + 8 * g, 8, t0 + nv, pos, low, p.sinks);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] = seen >> i & 1 ? s[i] : -INFINITY;
+      for (int i = 0; i < 8; ++i) s[i] = seen_or(seen, i, s[i]);
     }
     weights<CACHED, 8>(s, 0.f, masked, w);
     u4 pw, px;
