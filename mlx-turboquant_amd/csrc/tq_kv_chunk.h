@@ -66,18 +66,17 @@ struct Chunk {
     const int i = j * CH_THREADS + threadIdx.x;
     if (EVEN || i < PIECES) put16(kx[j], kl + krow(i / (D / 16)) * KP + i % (D / 16) * 16);
   }
-  // fp16: times `pw`, the powers of two of the tile's four groups of 16 tokens
-  __device__ void store_v8(const float (&pw)[4], uint16_t* vl, int j) const {
+  // fp16: times `power`, the power of two of this lane's 16 tokens (lane & 3)
+  __device__ void store_v8(float power, uint16_t* vl, int j) const {
     const int i = j * CH_THREADS + threadIdx.x;
     if (!EVEN && i >= PIECES) return;
-    const int c = i % (TILE / 16);
-    uint16_t* d = vl + i / (TILE / 16) * VP + c * 16;
+    uint16_t* d = vl + i / (TILE / 16) * VP + i % (TILE / 16) * 16;
     if constexpr (BF) {
       put16(vx[j], d);
     } else {
       const u4 x = vx[j];
       const u2 a = codes4<FMT, BF>(x.x), b = codes4<FMT, BF>(x.y), e = codes4<FMT, BF>(x.z), f = codes4<FMT, BF>(x.w);
-      const _Float16 s = (_Float16)(c & 2 ? c & 1 ? pw[3] : pw[2] : c & 1 ? pw[1] : pw[0]);
+      const _Float16 s = (_Float16)power;
       const h8 sc = {s, s, s, s, s, s, s, s};
       *(u4*)d = __builtin_bit_cast(u4, __builtin_bit_cast(h8, u4{a.x, a.y, b.x, b.y}) * sc);
       *(u4*)(d + 8) = __builtin_bit_cast(u4, __builtin_bit_cast(h8, u4{e.x, e.y, f.x, f.y}) * sc);
@@ -274,22 +273,23 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(cons
 
   // What 16 tokens of codes each have: sc multiplies scores, lf is log2 of what
   // multiplies weights, rf its inverse for their sum (a scale of 0 has codes of 0
-  // only: 1 will do).
+  // only: 1 will do). Lane & 3 has the scales of its 16 tokens; they become
+  // uniform only here.
   struct Scales {
     float sc[4], lf[4], rf[4];
   };
-  const auto scales_of = [&](int t0, bool codes) {
+  const auto scales_of = [&](bool codes, float ks, float vs) {
     Scales x;
+    if (codes) {
+      const float f = C::value_factor(vs);
+      const float sc = ks == 0.f ? scale : scale * ks, lf = __builtin_amdgcn_logf(f);
+      const float rf = f == f ? __builtin_amdgcn_rcpf(f) : 1.f;
+      const auto at = [](float y, int g) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(y), g)); };
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      x.sc[g] = scale, x.lf[g] = 0.f, x.rf[g] = 1.f;
-      if (codes) {
-        const int blk = (t0 + 16 * g) >> p.block_shift;
-        const float ks = ksc[blk], f = C::value_factor(vsc[blk]);
-        x.sc[g] = ks == 0.f ? scale : scale * ks;
-        x.lf[g] = __builtin_amdgcn_logf(f);
-        x.rf[g] = f == f ? __builtin_amdgcn_rcpf(f) : 1.f;
-      }
+      for (int g = 0; g < 4; ++g) x.sc[g] = at(sc, g), x.lf[g] = at(lf, g), x.rf[g] = at(rf, g);
+    } else {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) x.sc[g] = scale, x.lf[g] = 0.f, x.rf[g] = 1.f;
     }
     return x;
   };
@@ -422,13 +422,22 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(cons
     };
     const auto k_at = [&](int j) { return lds + (j & 1) * C::BUF; };
     const auto v_at = [&](int j) { return lds + (j & 1) * C::BUF + TILE * C::KP; };
+    // the scales of this lane's 16 tokens of tiles j and j + 1
+    float ks = 1.f, vs = 1.f, ks1 = 1.f, vs1 = 1.f;
+    const auto load_scales = [&](int j) {
+      if constexpr (CACHED) {
+        const int blk = (tile_at(j) * TILE + 16 * (lane & 3)) >> p.block_shift;
+        ks1 = ksc[blk];
+        vs1 = vsc[blk];
+      }
+    };
     // piece i of the C::PK + C::PV of tile j's keys and values
-    const auto store = [&](int j, int i, const float (&pw)[4]) -> uint32_t {
+    const auto store = [&](int j, int i) -> uint32_t {
       if constexpr (CACHED) {
         if (i < C::PK)
           c.store_k8(k_at(j), i);
         else
-          c.store_v8(pw, v_at(j), i - C::PK);
+          c.store_v8(C::value_power(vs1), v_at(j), i - C::PK);
         return 0;
       } else {
         if (i < C::PK) {
@@ -437,11 +446,6 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(cons
         }
         return c.template store_v16<C::AS_IS>(v_at(j), i - C::PK);
       }
-    };
-    const auto powers = [&](int j, float (&pw)[4]) {
-      if constexpr (CACHED && !BF)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) pw[g] = C::value_power(vsc[(tile_at(j) * TILE + 16 * g) >> p.block_shift]);
     };
     // what store left: apart from its straight line of code
     const auto mend_v = [&](int j, uint32_t found) {
@@ -454,28 +458,32 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(cons
         for (int i = 0; i < C::PV; ++i) c.template store_v16<C::FINITE>(v_at(j), i);
       }
     };
-    float pw[4];
     uint32_t found = 0;
+    load_scales(0);
     load_k(0);
     load_v(0);
-    powers(0, pw);
 #pragma unroll
-    for (int i = 0; i < C::PK + C::PV; ++i) found = top16(found, store(0, i, pw));
+    for (int i = 0; i < C::PK + C::PV; ++i) found = top16(found, store(0, i));
+    ks = ks1;
+    vs = vs1;
+    load_scales(1);
     load_k(1);
     mend_v(0, found);
     load_v(1);
     for (int j = 0; j < count; ++j) {
       const int t0 = tile_at(j) * TILE;
-      Scales x = scales_of(t0, CACHED);
+      Scales x = scales_of(CACHED, ks, vs);
       __syncthreads();
       f16v s[2];
       found = 0;
-      powers(j + 1, pw);
       scores(s, k_at(j), [&](int r) {  // the pieces spread over the NS / 2 groups of products
 #pragma unroll
         for (int i = 0; i < C::PK + C::PV; ++i)
-          if (i * (NS / 2) / (C::PK + C::PV) == r) found = top16(found, store(j + 1, i, pw));
+          if (i * (NS / 2) / (C::PK + C::PV) == r) found = top16(found, store(j + 1, i));
       });
+      ks = ks1;
+      vs = vs1;
+      load_scales(j + 2);
       load_k(j + 2);
       mend_v(j + 1, found);
       load_v(j + 2);
@@ -491,7 +499,7 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(cons
     __syncthreads();
     f16v s[2];
     scores(s, lds, [](int) {});
-    Scales x = scales_of(tl.main_len, false);
+    Scales x = scales_of(false, 1.f, 1.f);
     before(s, x, tl.main_len, nv);
     output(s, x, vl);
   }
