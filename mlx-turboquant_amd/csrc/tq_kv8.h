@@ -160,6 +160,15 @@ __device__ inline uint32_t seen2(uint32_t bits) {
   return (bits & 1u ? one : 0u) | (bits & 2u ? one << 16 : 0u);
 }
 
+// acc plus both elements.
+template <bool BF>
+__device__ inline float add2(uint32_t x, float acc) {
+  if constexpr (BF)
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, x), b2{(__bf16)1.f, (__bf16)1.f}, acc, false);
+  else
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, x), h2{(_Float16)1.f, (_Float16)1.f}, acc, false);
+}
+
 template <bool BF>
 __device__ inline f4 mma16(u4 a, u4 b, f4 c) {
   if constexpr (BF)

@@ -338,17 +338,21 @@ __global__ __launch_bounds__(WAVES * 64, D > 128 ? 1 : 2) void chunk_kernel(cons
       m = mn;
     }
   };
-  // Weights of 16 tokens (8 of them this lane's).
+  // Weights of 16 tokens (8 of them this lane's). Their sum is that of the rounded
+  // ones: a weight's rounding then moves the output by its distance from that
+  // token's value only (a lone weight cancels), and two are added at once.
   const auto weights = [&](const f16v (&s)[2], const Scales& x, int g) {
     const float off = x.lf[g] - (m == -INFINITY ? 0.f : m);
-    float w[8], sum = 0.f;
+    float sum = 0.f;
+    u4 w;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      w[k] = __builtin_amdgcn_exp2f(fmaf(s[g >> 1][(g & 1) * 8 + k], x.sc[g], off));
-      sum += w[k];
+    for (int k = 0; k < 4; ++k) {
+      const int i = (g & 1) * 8 + 2 * k;
+      w[k] = bits2<BF>(__builtin_amdgcn_exp2f(fmaf(s[g >> 1][i], x.sc[g], off)), __builtin_amdgcn_exp2f(fmaf(s[g >> 1][i + 1], x.sc[g], off)));
+      sum = add2<BF>(w[k], sum);
     }
     l = fmaf(sum, x.rf[g], l);
-    return u4{bits2<BF>(w[0], w[1]), bits2<BF>(w[2], w[3]), bits2<BF>(w[4], w[5]), bits2<BF>(w[6], w[7])};
+    return w;
   };
   // Other work goes between the products, a few instructions each: what runs
   // under a product (they do not run beside another wave's).

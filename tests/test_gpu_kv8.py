@@ -538,6 +538,26 @@ def test_steps_of_a_batch_equal_single_sequences():
     assert batch.offset.tolist() == [n + steps for n in prompts] == batch.lens.tolist()
 
 
+def test_batch_with_windows_drafts_and_outputs():
+    from turboquant_amd import KV8Batch, kv8_attention
+    B, H, hq, D = 3, 2, 6, 64
+    batch = KV8Batch(B, H, D, "fp8", 16, capacity=64, window=20, sinks=3)
+    assert (batch.attend(rand(150, B, hq, D)) == 0).all()  # nothing in it yet
+    for b, n in enumerate((5, 130, 0)):
+        if n:
+            batch.load(b, rand(151 + b, H, n, D), rand(161 + b, H, n, D))
+    for i in range(4):
+        batch.step(rand(170 + i, B, H, D), rand(180 + i, B, H, D))
+    assert batch.lens.tolist() == [9, 134, 4] and batch.store.cap >= 134
+    q = rand(190, B, hq, 4, D)
+    want = kv8_attention(q, batch.store, batch.lens, 134, None, 20, 3)
+    assert torch.equal(batch.attend(q), want)
+    last = batch.attend(q[:, :, -1])
+    assert last.shape == (B, hq, D) and torch.allclose(last.float(), want[:, :, -1].float(), rtol=2 ** -9, atol=2 ** -12)
+    out = torch.empty(B, hq, D, dtype=torch.float32, device=DEV)
+    assert batch.attend(q[:, :, -1], out=out).data_ptr() == out.data_ptr() and torch.equal(out.half(), last)
+
+
 def test_captured_step_replays():
     """A decode step (write, length, attention) in a HIP graph, replayed over block borders with eager work between, two graphs
     on their own streams at once: every replay as the eager step."""
