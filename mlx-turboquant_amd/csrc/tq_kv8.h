@@ -184,17 +184,38 @@ __device__ inline f16v mma32(u4 a, u4 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
 
-// The maximum over the lanes that differ in bits 4 and 5 (16) or 5 (32)
-// of their number, without a trip through LDS.
+// Reductions over a wave without trips through LDS: rotations within rows of 16
+// lanes, then exchanges of rows and of halves. Every lane gets the result.
+template <int N>
+__device__ inline uint32_t row_rotated(uint32_t x) {
+  return __builtin_amdgcn_update_dpp(0, x, 0x120 + N, 0xf, 0xf, true);
+}
+template <typename F>
+__device__ inline uint32_t rows_joined(uint32_t x, F f) {  // over the lanes that differ in bits 4 and 5
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = f(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return f(b[0], b[1]);
+}
+template <typename F>
+__device__ inline uint32_t wave_joined(uint32_t x, F f) {
+  x = f(x, row_rotated<8>(x));
+  x = f(x, row_rotated<4>(x));
+  x = f(x, row_rotated<2>(x));
+  x = f(x, row_rotated<1>(x));
+  return rows_joined(x, f);
+}
+__device__ inline uint32_t max_bits(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+__device__ inline uint32_t sum_bits(uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }
+__device__ inline float wave_max(float x) { return __uint_as_float(wave_joined(__float_as_uint(x), max_bits)); }
+__device__ inline float wave_sum(float x) { return __uint_as_float(wave_joined(__float_as_uint(x), sum_bits)); }
+
+// The maximum over the lanes that differ in bits 4 and 5 (16) or 5 (32) of their
+// number.
 template <int FROM>
 __device__ inline float lanes_max(float x) {
-  uint32_t v = __float_as_uint(x);
-  if constexpr (FROM == 16) {
-    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    v = __float_as_uint(x);
-  }
-  const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  if constexpr (FROM == 16) return __uint_as_float(rows_joined(__float_as_uint(x), max_bits));
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 

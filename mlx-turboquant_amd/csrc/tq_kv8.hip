@@ -76,8 +76,7 @@ __global__ __launch_bounds__(WT) void write_kernel(const WriteParams p) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) top = top16(top, x[i][k]);
       top = max(top & 0xffffu, top >> 16);
-#pragma unroll
-      for (int k = 1; k < 64; k *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, k));
+      top = wave_joined(top, [](uint32_t a, uint32_t b) { return max(a, b); });
       const int w = i * (WT / 64) + wave;  // 64 pieces; 2 D of them are 16 tokens
       if (lane == 0) part[w / PARTS][w % PARTS] = top;
     }
@@ -87,6 +86,7 @@ __global__ __launch_bounds__(WT) void write_kernel(const WriteParams p) {
 #pragma unroll
     for (int g = 0; g < TILE / BLOCK; ++g) {
       uint32_t top = 0;
+#pragma unroll
       for (int k = 0; k < BLOCK / 16 * PARTS; ++k) top = max(top, part[g * (BLOCK / 16) + k / PARTS][k % PARTS]);
       const float a = elem<BF>(top);
       const bool finite = top < (BF ? 0x7f80u : 0x7c00u), codes = finite && a >= TINY;
