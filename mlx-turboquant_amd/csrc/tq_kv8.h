@@ -289,14 +289,14 @@ __device__ inline int decode_places(const Params& p, bool cached, int b) {
   return (n + DEC_WAVES - 1) / DEC_WAVES * DEC_WAVES;
 }
 
-// Inclusive sums over the wave's lanes.
-__device__ inline int wave_scan(int n, int lane) {
-#pragma unroll
-  for (int k = 1; k < 64; k *= 2) {
-    const int up = __shfl_up(n, k);
-    if (lane >= k) n += up;
-  }
-  return n;
+// Inclusive sums over the wave's lanes: within rows of 16, then the rows before.
+__device__ inline int wave_scan(int n) {
+  n += __builtin_amdgcn_update_dpp(0, n, 0x111, 0xf, 0xf, false);  // row_shr:1, 2, 4, 8
+  n += __builtin_amdgcn_update_dpp(0, n, 0x112, 0xf, 0xf, false);
+  n += __builtin_amdgcn_update_dpp(0, n, 0x114, 0xf, 0xf, false);
+  n += __builtin_amdgcn_update_dpp(0, n, 0x118, 0xf, 0xf, false);
+  n += __builtin_amdgcn_update_dpp(0, n, 0x142, 0xa, 0xf, false);  // row_bcast:15 to rows 1 and 3, :31 to 2 and 3
+  return n + __builtin_amdgcn_update_dpp(0, n, 0x143, 0xc, 0xf, false);
 }
 
 // The share, and for workgroup `wg` (>= 0) the sequence that its first tile
@@ -316,11 +316,11 @@ __device__ inline Share share_of(const Params& p, bool cached, int wg, int& b, i
     return s;
   }
   int n = lane < p.batch ? decode_places(p, cached, lane) * p.hkv : 0;
-  int sum = wave_scan(n, lane);  // of the first 64 sequences
-  int total = __shfl(sum, 63);
+  int sum = wave_scan(n);  // of the first 64 sequences
+  int total = __builtin_amdgcn_readlane(sum, 63);
   for (int b0 = 64; b0 < p.batch; b0 += 64)
-    total += __shfl(wave_scan(b0 + lane < p.batch ? decode_places(p, cached, b0 + lane) * p.hkv : 0, lane), 63);
-  per_of(__builtin_amdgcn_readfirstlane(total));
+    total += __builtin_amdgcn_readlane(wave_scan(b0 + lane < p.batch ? decode_places(p, cached, b0 + lane) * p.hkv : 0), 63);
+  per_of(total);
   const int at = wg * s.per;
   if (wg >= 0 && at >= s.total) {
     b = -1;
@@ -336,14 +336,13 @@ __device__ inline Share share_of(const Params& p, bool cached, int wg, int& b, i
       l = b - b0;
     }
     if (l >= 0) {
-      if (l > 0) base += __shfl(sum, l - 1);
-      before = __builtin_amdgcn_readfirstlane(base);
-      b = __builtin_amdgcn_readfirstlane(b0 + l);
+      before = base + (l > 0 ? __builtin_amdgcn_readlane(sum, l - 1) : 0);
+      b = b0 + l;
       return s;
     }
-    base += __shfl(sum, 63);
+    base += __builtin_amdgcn_readlane(sum, 63);
     n = b0 + 64 + lane < p.batch ? decode_places(p, cached, b0 + 64 + lane) * p.hkv : 0;
-    sum = wave_scan(n, lane);
+    sum = wave_scan(n);
   }
 }
 

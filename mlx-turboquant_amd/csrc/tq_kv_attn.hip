@@ -24,7 +24,7 @@ extern template hipError_t launch_chunk<256>(const Params&, bool, int, hipStream
 
 namespace {
 
-constexpr int MT = 512;
+constexpr int MT = 256;
 // Workgroups that share the tiles in decode: two per CU, what their registers
 // allow.
 constexpr int STREAM_WGS = 512;
@@ -39,13 +39,13 @@ constexpr int DIRECT_WORK = 2816;
 template <int D, bool BF>
 __global__ __launch_bounds__(MT) void merge_kernel(const Params p, bool cached) {
   // Lanes of 4 dims, groups of partials (D = 96: some threads idle). Latency bounds
-  // it, so the partials go by 64: every wave works out their weights by itself, one to
-  // a lane, while a thread's N pieces of them are on their way. Against weights first
-  // and 256 threads, calls as a whole: 131072 tokens, 8 kv heads 66.3 -> 63.6 us; 4
-  // tokens to each of 8 sequences of up to 4K, head dim 256, 28.8 -> 27.6; 32 sequences
-  // of up to 16K, where a row has two or three partials, 119.7 -> 120.7 (256 threads
-  // and this order: 122).
-  constexpr int L = D / 4, G = MT / L, N = (64 + G - 1) / G;
+  // it, so every wave works out the weights of PASS partials by itself, one to a lane,
+  // while a thread's N pieces of them are on their way. Threads (MT) 64 / 128 / 256 /
+  // 512, us of the calls as a whole: 131072 tokens, 8 kv heads 64.8 / 63.3 / 62.7 /
+  // 62.8; 4 tokens to each of 8 sequences of up to 4K, head dim 256, 28.3 / 27.7 / 27.3
+  // / 27.4; 32 sequences of up to 16K, where a row has two or three partials, 118.4 /
+  // 118.7 / 119.5 / 121.1.
+  constexpr int L = D / 4, G = MT / L, PASS = G < 8 ? 8 * G : 64, N = (PASS + G - 1) / G;
   __shared__ f4 os[G][L];
   const int unit = blockIdx.x;
   const int bh = unit / p.rows, row = unit - bh * p.rows;
@@ -76,8 +76,8 @@ __global__ __launch_bounds__(MT) void merge_kernel(const Params p, bool cached) 
   const float* o = p.ws + p.o_off + slot * D + c * 4;
   float Mr = 0.f, mr = 0.f, l = 0.f;
   f4 x = {0.f, 0.f, 0.f, 0.f};
-  for (int i0 = 0; i0 < count; i0 += 64) {
-    const int n = min(64, count - i0);
+  for (int i0 = 0; i0 < count; i0 += PASS) {
+    const int n = min(PASS, count - i0);
     f4 y[N];
 #pragma unroll
     for (int j = 0; j < N; ++j)
