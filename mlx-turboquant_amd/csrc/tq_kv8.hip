@@ -11,8 +11,8 @@
 // call's first tile also moves the incomplete block: it has read the tail before
 // it writes there.
 //
-// Measured, 8 kv heads, head dim 128, bf16, int8: 8192 tokens written in 14.6 us
-// (3.5 TB/s; 2.6 us for one token), 32,768 read back in 31.5 us (6.4 TB/s).
+// Measured, 8 kv heads, head dim 128, bf16, int8: 8192 tokens written in 13.3 us
+// (3.8 TB/s; 2.8 us for one token), 32,768 read back in 32.0 us (6.3 TB/s).
 
 #include "tq_kv8.h"
 

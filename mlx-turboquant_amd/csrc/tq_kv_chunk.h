@@ -8,10 +8,10 @@
 // vector instructions bound it together: on this chip their times add up but for
 // about two vector instructions per product. So each step has as few of them as
 // could be found, spread between the products: per wave and tile of codes at
-// head dim 128, 32 products and 253 others, 32 of them exponentials.
+// head dim 128, 32 products and 244 others, 32 of them exponentials.
 //
 // Measured: 2048 queries of 32 heads on 8 over 32,768 tokens, head dim 128, bf16,
-// int8: 1041 us, 1.02 PFLOP/s (a large bf16 product reaches 1.22); 8192 queries
+// int8: 1028 us, 1.04 PFLOP/s (a large bf16 product reaches 1.22); 8192 queries
 // over 16-bit keys and values, window 1024: 190 us, 0.68 PFLOP/s of what is seen.
 //
 // Scores, transposed: S^T = K q^T. Key row m of a 32-token half tile is token m
