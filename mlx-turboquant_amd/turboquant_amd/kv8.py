@@ -315,7 +315,8 @@ def kv8_attention(queries: torch.Tensor, store: KV8Store, lens, max_len: int | N
     sequence, or one shorter than T_q) gives 0. Default scale D**-0.5.
 
     Returns (B, Hq, T_q, D) of the queries' type, or ``out`` (that type or
-    float32, any strides that are multiples of 8). Scores, softmax and sums are
+    float32, any strides that are multiples of 8; the queries
+    themselves may be given). Scores, softmax and sums are
     float32; the softmax's weights are rounded to 16 bits. (Sums of query times
     code must stay in float32's range: with more than 16 query rows per kv head,
     bf16 queries below 2**112.)"""

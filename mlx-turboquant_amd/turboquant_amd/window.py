@@ -32,7 +32,8 @@ def window_attention(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
 
     Returns (B, Hq, T_q, D) of the queries' type, or ``out`` (that type or
     float32). Scores, softmax and sums are float32; the softmax's weights are
-    rounded to 16 bits (bf16 with few query rows: to two parts)."""
+    rounded to 16 bits (bf16 with few query rows: to two parts). For inference:
+    no gradients."""
     if keys.dim() != 4 or values.shape != keys.shape or values.dtype != keys.dtype or values.device != keys.device:
         raise ValueError("keys and values must have one shape (B, Hkv, T, D), dtype and device")
     B, H, T, D = keys.shape

@@ -622,6 +622,42 @@ def test_streams():
     assert torch.equal(got, want) and torch.equal(r, wr)
 
 
+@pytest.mark.parametrize("lens", [(40000,), (20011, 0, 12000)], ids=str)
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+def test_one_head_over_many_workgroups(D, lens):
+    """A row whose parts are more than the join takes at once, in whole caches and ragged ones."""
+    from turboquant_amd import kv8_attention, window_attention
+    B, T, block = len(lens), max(lens), 32
+    k, v, q = rand(94, B, 1, T, D), rand(95, B, 1, T, D, scale=2.0), rand(96, B, 3, 1, D, scale=1.5)
+    v[:, :, :T // 2] *= 1e-3  # parts of unlike scales
+    store = store_of(k, "int8", block, T, v)
+    for b, n in enumerate(lens):
+        full = n // block * block
+        store.k_tail[b, :, :n - full], store.v_tail[b, :, :n - full] = k[b, :, full:n], v[b, :, full:n]
+    lt = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    calls = [lt] if B > 1 else [lt, lens[0]]
+    for n_arg in calls:
+        got = kv8_attention(q, store, n_arg)
+        dense = window_attention(q, k, v, lens=n_arg)
+        for b, n in enumerate(lens):
+            want, tol = attend(q[b], exact_tokens(k[b], n, "int8", block), exact_tokens(v[b], n, "int8", block), n, 0, 0,
+                               weights=torch.float16) if n else (torch.zeros(3, 1, D), torch.zeros(3, 1, D))
+            check(got[b], want.double(), tol.double(), q.dtype, f"8-bit, sequence {b}")
+            want, tol = attend(q[b], k[b, :, :n], v[b, :, :n], n, 0, 0, weights=torch.float16) if n else (want, tol)
+            check(dense[b], want.double(), tol.double(), q.dtype, f"16-bit, sequence {b}")
+
+
+@pytest.mark.parametrize("B,H,T,nq", [(1, 2, 300, 1), (1, 2, 6000, 1), (2, 2, 6000, 3), (1, 2, 900, 70), (32, 8, 200, 20)])
+def test_output_over_the_queries(B, H, T, nq):
+    """``out`` may be the queries themselves."""
+    from turboquant_amd import kv8_attention, window_attention
+    k, q = rand(97, B, H, T, 64), rand(98, B, 2 * H, nq, 64)
+    store = store_of(k, "fp8", 16, T)
+    for call in (lambda x, **a: kv8_attention(x, store, T, **a), lambda x, **a: window_attention(x, k, k, **a)):
+        want, mine = call(q), q.clone()
+        assert call(mine, out=mine) is mine and torch.equal(mine, want)
+
+
 def test_repeatable():
     """The same call gives the same bits (no atomics)."""
     from turboquant_amd import kv8_attention
