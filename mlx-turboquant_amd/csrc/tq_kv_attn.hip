@@ -29,10 +29,11 @@ constexpr int MT = 256;
 // allow.
 constexpr int STREAM_WGS = 512;
 // One workgroup per (sequence, kv head) and no merge instead, up to so many
-// tiles times head dim. Decode and merge against that, us, 8 kv heads, bf16,
-// int8: 1024 tokens 16.4 / 13.7 at head dim 128 and 17.3 / 9.5 at 64; 1536
-// tokens 16.3 / 16.8 at 128; 1024 tokens 18.4 / 27.5 at 256.
-constexpr int DIRECT_WORK = 2816;
+// tiles (the incomplete block's among them) times head dim. Split and merged
+// against that, us, one sequence of 8 kv heads, bf16, int8: head dim 64, 1024
+// tokens 9.4 / 8.4, 1536 9.4 / 10.6; 128, 512 tokens 11.4 / 9.1, 1024 11.4 /
+// 13.1; 256, 256 tokens 16.8 / 12.8, 512 17.1 / 18.4; 8 sequences alike.
+constexpr int DIRECT_WORK = 1536;
 
 // One query row per workgroup: the partials (M, m, l, O) of its splits, O in
 // units of 2^M, l in units of 2^m, to out = 2^(M - m) O / l.
@@ -184,7 +185,7 @@ int plan(const tq_kv8_store* s, const tq_kv_attn_desc* d, Params& p, bool& decod
   if (decode) {
     p.wgs = 0;
     // also where units of one length fill the chip evenly: 64 sequences of 4096
-    // tokens, head dim 128: 94.7 us against 102
+    // tokens, head dim 128: 94.6 us against 102.8
     const bool even = d->len_b == nullptr && units % STREAM_WGS == 0;
     if (tiles * d->d > DIRECT_WORK && !even) p.wgs = (int)std::min<int64_t>(STREAM_WGS, units * ((tiles + DEC_WAVES - 1) / DEC_WAVES));
     if (p.wgs) slots = (p.wgs + units) * p.rows;
