@@ -25,6 +25,11 @@ extern template hipError_t launch_chunk<256>(const Params&, bool, int, hipStream
 namespace {
 
 constexpr int MT = 256;
+// Up to so many splits of a chunk, several rows per workgroup join theirs. One row
+// per workgroup against that, us, 32 heads of head dim 128 over 4096 tokens: 1024
+// queries in 2 splits 147 / 92, 128 in 8 splits 37.1 / 32.4, 32 in 8 splits 25.9 /
+// 26.4, in 16 splits 22.1 / 24.7.
+constexpr int ROWS_SPLITS = 8;
 // Workgroups that share the tiles in decode: two per CU, what their registers
 // allow.
 constexpr int STREAM_WGS = 512;
@@ -35,8 +40,82 @@ constexpr int STREAM_WGS = 512;
 // 13.1; 256, 256 tokens 16.8 / 12.8, 512 17.1 / 18.4; 8 sequences alike.
 constexpr int DIRECT_WORK = 1536;
 
-// One query row per workgroup: the partials (M, m, l, O) of its splits, O in
-// units of 2^M, l in units of 2^m, to out = 2^(M - m) O / l.
+// Where a query row's partials (M, m, l, O) lie, O in units of 2^M, l in units of
+// 2^m; joined they give out = 2^(M - m) O / l.
+struct MergeRow {
+  int b, h, qi, head, len;
+  int count;           // partials
+  int64_t slot, step;  // first partial, distance of the next
+};
+
+// A row of chunks that are split: its own slots, one after the other.
+__device__ inline MergeRow chunk_row(const Params& p, bool cached, int unit) {
+  MergeRow r;
+  const int bh = unit / p.rows, row = unit - bh * p.rows;
+  r.b = bh / p.hkv, r.h = bh - r.b * p.hkv;
+  r.qi = row / p.group, r.head = row - r.qi * p.group;
+  r.len = length_of(p, r.b);
+  const int r0 = row / p.tile_rows * p.tile_rows;
+  const int pmin = r.len - p.n_q + r0 / p.group, pmax = r.len - p.n_q + min(p.rows - 1, r0 + p.tile_rows - 1) / p.group;
+  r.count = (tiles_of(r.len, cached, p.block_shift, pmin, pmax, p.window, p.sinks).n + p.chunk - 1) / p.chunk;
+  r.slot = (int64_t)unit * p.splits;
+  r.step = 1;
+  return r;
+}
+
+// A row of decode, whose slots lie one for each workgroup that shares its unit.
+__device__ inline MergeRow shared_row(const Params& p, bool cached, int unit) {
+  MergeRow r;
+  const int bh = unit / p.rows, row = unit - bh * p.rows;
+  r.b = bh / p.hkv, r.h = bh - r.b * p.hkv;
+  r.qi = row / p.group, r.head = row - r.qi * p.group;
+  r.len = length_of(p, r.b);
+  int seq = r.b, before;
+  const Share sh = share_of(p, cached, -1, seq, before);
+  const int n = decode_places(p, cached, r.b), at = before + r.h * n;
+  r.count = n ? (at + n - 1) / sh.per - at / sh.per + 1 : 0;
+  r.slot = (int64_t)(at / sh.per + bh) * p.rows + row;
+  r.step = p.rows;
+  return r;
+}
+
+// 4 dims of the row: the partials' sums x and l.
+template <bool BF>
+__device__ inline void put_row(const Params& p, const MergeRow& r, int c, f4 x, float l, float Mr, float mr) {
+  const float inv = 1.f / l, f = __builtin_amdgcn_exp2f(Mr - mr);  // apart: their product can be subnormal
+  x = r.len - p.n_q + r.qi < 0 ? f4{0.f, 0.f, 0.f, 0.f} : x * inv * f;
+  const int64_t at = (int64_t)r.b * p.out.sb + (int64_t)(r.h * p.group + r.head) * p.out.sh + (int64_t)r.qi * p.out.st + c * 4;
+  if (p.out_f32)
+    *(f4*)((float*)p.out.p + at) = x;
+  else
+    *(u2*)((uint16_t*)p.out.p + at) = u2{bits2<BF>(x[0], x[1]), bits2<BF>(x[2], x[3])};
+}
+
+// Rows of chunks in few splits: D / 4 threads per row, one partial after another,
+// two at a time on their way. Bound by the partials' bytes.
+template <int D, bool BF>
+__global__ __launch_bounds__(MT) void merge_rows_kernel(const Params p, bool cached, int units) {
+  constexpr int L = D / 4, R = MT / L;
+  const int c = threadIdx.x % L, i0 = threadIdx.x / L;
+  const int64_t unit = (int64_t)blockIdx.x * R + i0;
+  if (i0 >= R || unit >= units) return;
+  const MergeRow r = chunk_row(p, cached, (int)unit);
+  const f4* ml = (const f4*)p.ws + r.slot;
+  const f4* o = (const f4*)(p.ws + p.o_off) + r.slot * L + c;
+  float M = -INFINITY, m = -INFINITY;
+  for (int i = 0; i < r.count; ++i) M = fmaxf(M, ml[i].x), m = fmaxf(m, ml[i].y);
+  const float Mr = M == -INFINITY ? 0.f : M, mr = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  f4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+  for (int i = 0; i < r.count; ++i) {
+    l += ml[i].z * __builtin_amdgcn_exp2f(ml[i].y - mr);
+    x += o[(int64_t)i * L] * __builtin_amdgcn_exp2f(ml[i].x - Mr);
+  }
+  put_row<BF>(p, r, c, x, l, Mr, mr);
+}
+
+// One query row per workgroup.
 template <int D, bool BF>
 __global__ __launch_bounds__(MT) void merge_kernel(const Params p, bool cached) {
   // Lanes of 4 dims, groups of partials (D = 96: some threads idle). Latency bounds
@@ -48,33 +127,14 @@ __global__ __launch_bounds__(MT) void merge_kernel(const Params p, bool cached) 
   // 118.7 / 119.5 / 121.1.
   constexpr int L = D / 4, G = MT / L, PASS = G < 8 ? 8 * G : 64, N = (PASS + G - 1) / G;
   __shared__ f4 os[G][L];
-  const int unit = blockIdx.x;
-  const int bh = unit / p.rows, row = unit - bh * p.rows;
-  const int b = bh / p.hkv, h = bh - b * p.hkv;
-  const int qi = row / p.group, head = row - qi * p.group;
-  const int len = length_of(p, b);
-  int count;
-  int64_t slot, step;  // first partial, distance of the next
-  if (p.wgs) {
-    int seq = b, before;
-    const Share sh = share_of(p, cached, -1, seq, before);
-    const int n = decode_places(p, cached, b), at = before + h * n;
-    count = n ? (at + n - 1) / sh.per - at / sh.per + 1 : 0;
-    slot = (int64_t)(at / sh.per + bh) * p.rows + row;
-    step = p.rows;
-  } else {
-    const int r0 = row / p.tile_rows * p.tile_rows;
-    const int pmin = len - p.n_q + r0 / p.group, pmax = len - p.n_q + min(p.rows - 1, r0 + p.tile_rows - 1) / p.group;
-    count = (tiles_of(len, cached, p.block_shift, pmin, pmax, p.window, p.sinks).n + p.chunk - 1) / p.chunk;
-    slot = (int64_t)unit * p.splits;
-    step = 1;
-  }
-  const float* ml = p.ws + slot * 4;
-  step *= 4;
+  const MergeRow r = p.wgs ? shared_row(p, cached, blockIdx.x) : chunk_row(p, cached, blockIdx.x);
+  const int count = r.count;
+  const float* ml = p.ws + r.slot * 4;
+  const int64_t step = r.step * 4;
 
   const int lane = threadIdx.x & 63, c = threadIdx.x % L, grp = threadIdx.x / L;
   float M = -INFINITY, m = -INFINITY;
-  const float* o = p.ws + p.o_off + slot * D + c * 4;
+  const float* o = p.ws + p.o_off + r.slot * D + c * 4;
   float Mr = 0.f, mr = 0.f, l = 0.f;
   f4 x = {0.f, 0.f, 0.f, 0.f};
   for (int i0 = 0; i0 < count; i0 += PASS) {
@@ -107,22 +167,24 @@ __global__ __launch_bounds__(MT) void merge_kernel(const Params p, bool cached) 
   if (threadIdx.x >= L) return;
 #pragma unroll
   for (int i = 1; i < G; ++i) x += os[i][c];
-  const float inv = 1.f / l, f = __builtin_amdgcn_exp2f(Mr - mr);  // apart: their product can be subnormal
-  x = len - p.n_q + qi < 0 ? f4{0.f, 0.f, 0.f, 0.f} : x * inv * f;
-  const int64_t at = (int64_t)b * p.out.sb + (int64_t)(h * p.group + head) * p.out.sh + (int64_t)qi * p.out.st + c * 4;
-  if (p.out_f32)
-    *(f4*)((float*)p.out.p + at) = x;
-  else
-    *(u2*)((uint16_t*)p.out.p + at) = u2{bits2<BF>(x[0], x[1]), bits2<BF>(x[2], x[3])};
+  put_row<BF>(p, r, c, x, l, Mr, mr);
 }
 
 template <int D>
 hipError_t launch_merge(const Params& p, bool bf16, bool cached, hipStream_t s) {
   const uint32_t units = (uint32_t)(p.batch * p.hkv * p.rows);
-  if (bf16)
+  if (p.wgs == 0 && p.splits <= ROWS_SPLITS) {
+    constexpr int R = MT / (D / 4);
+    const uint32_t wgs = (units + R - 1) / R;
+    if (bf16)
+      merge_rows_kernel<D, true><<<wgs, MT, 0, s>>>(p, cached, (int)units);
+    else
+      merge_rows_kernel<D, false><<<wgs, MT, 0, s>>>(p, cached, (int)units);
+  } else if (bf16) {
     merge_kernel<D, true><<<units, MT, 0, s>>>(p, cached);
-  else
+  } else {
     merge_kernel<D, false><<<units, MT, 0, s>>>(p, cached);
+  }
   return hipGetLastError();
 }
 
