@@ -188,6 +188,42 @@ hipError_t launch_merge(const Params& p, bool bf16, bool cached, hipStream_t s) 
   return hipGetLastError();
 }
 
+// Rows per workgroup of the chunk kernel, 128 (4 waves, two workgroups per CU up to
+// head dim 128) or 256 (8 waves, which share each tile's way through LDS), and in how
+// many parts a row tile's key tiles go to workgroups of their own: the pair of the
+// least estimated time. Workgroups run in rounds of one or two per CU; a round takes
+// as long as its share of tiles, and as 4 more for its beginning and end; parts are
+// written and read again. Times are in those of a tile of 128 rows alone on a CU,
+// 0.37 + 0.0066 head dim us: 1.5 for two beside each other, 1.45 for one of 256 rows.
+//
+// Candidates are the most parts that fill one to four rounds. us, 32 heads on 8, bf16,
+// int8, head dim 128, 128 rows unsplit / 128 rows in 2 to 4 parts / 256 rows unsplit /
+// 256 rows in parts that fill two or three rounds: 768 queries over 32,768 tokens 681 /
+// 417 / - / 391, 1280 queries 993 / 684 / 901 / 626, 1536 994 / 806 / 900 / 721, 2048
+// 995 / 1019 / 902 / 930; 1024 over 4096 92 / 88 / 122 / 83. 8192 queries over 16-bit
+// keys and values, unsplit: window 1024 192 / - / 197, 2048 327 / - / 316. Over the 28 shapes that
+// were timed the choice is 0.8% off the best on average, 8% at most.
+template <typename F>
+void choose_chunks(int64_t heads, int64_t rows, int d, const F& most_tiles, int& tile_rows, int& splits) {
+  constexpr int CUS = 256;
+  const double tile_us = 0.37 + 0.0066 * d;
+  double best = INFINITY;
+  for (int r = 128; r <= (d <= 128 ? 256 : 128); r *= 2) {
+    const bool two = r == 128 && d <= 128;
+    const int64_t tiles = most_tiles(r), base = std::max<int64_t>(1, heads * ((rows + r - 1) / r));
+    for (int round = 0; round <= 4; ++round) {
+      const int64_t want = round ? std::min(CUS * round / base, (tiles + 3) / 4) : 1;
+      if (want < 1 || (round && want == 1)) continue;
+      const int64_t chunk = (tiles + want - 1) / want, parts = (tiles + chunk - 1) / chunk;
+      const int64_t wgs = base * parts, full = wgs / (two ? 2 * CUS : CUS), rest = wgs % (two ? 2 * CUS : CUS);
+      const double time = two ? 1.5 * (full + (rest > CUS)) + (rest > 0 && rest <= CUS) : (r == 256 ? 1.45 : 1.0) * (full + (rest > 0));
+      double us = time * (chunk + 4) * tile_us;
+      if (parts > 1) us += 4 + 8e-6 / 5 * (d + 4) * (double)(heads * rows * parts);  // the merge; bytes at 5 TB/s
+      if (us < best) best = us, tile_rows = r, splits = (int)parts;
+    }
+  }
+}
+
 // Shapes of a call; fills what the launch needs but the pointers.
 int plan(const tq_kv8_store* s, const tq_kv_attn_desc* d, Params& p, bool& decode, size_t& bytes) {
   if (d == nullptr) return set_error(TQ_ERR_INVALID, "attention: NULL descriptor");
@@ -231,13 +267,9 @@ int plan(const tq_kv8_store* s, const tq_kv_attn_desc* d, Params& p, bool& decod
     }
     return std::max<int64_t>(1, tiles + (s != nullptr));
   };
-  // Rows per workgroup of the chunk kernel. 256 (one workgroup of 8 waves per
-  // CU) share each tile's way through LDS among twice the rows, where they still
-  // fill the chip and have many tiles (8192 bf16 queries of 32 heads on 8, head
-  // dim 128: window 8192 1088 us against 1177 for 128, 2048 316 against 327);
-  // with few, two workgroups of 4 waves per CU hide each other's beginnings and
-  // ends (window 1024: 192 us against 197).
-  p.tile_rows = d->d <= 128 && heads * ((p.rows + 255) / 256) >= 256 && most_tiles(256) >= 32 ? 256 : 128;
+  p.tile_rows = 128;
+  p.splits = 1;
+  if (!decode) choose_chunks(heads, p.rows, d->d, most_tiles, p.tile_rows, p.splits);
   p.row_tiles = decode ? 1 : (p.rows + p.tile_rows - 1) / p.tile_rows;
   const int64_t tiles = most_tiles(decode ? p.rows : p.tile_rows);
   const int64_t units = heads, base = units * p.row_tiles;
@@ -252,10 +284,7 @@ int plan(const tq_kv8_store* s, const tq_kv_attn_desc* d, Params& p, bool& decod
     if (tiles * d->d > DIRECT_WORK && !even) p.wgs = (int)std::min<int64_t>(STREAM_WGS, units * ((tiles + DEC_WAVES - 1) / DEC_WAVES));
     if (p.wgs) slots = (p.wgs + units) * p.rows;
   } else {
-    int64_t splits = base > 0 && base < 256 ? (512 + base - 1) / base : 1;
-    const int64_t most = (tiles + 3) / 4;
-    if (splits > most) splits = most;
-    p.chunk = (int)((tiles + splits - 1) / splits);
+    p.chunk = (int)((tiles + p.splits - 1) / p.splits);
     p.splits = (int)((tiles + p.chunk - 1) / p.chunk);
     if (base * p.splits >= (int64_t)1 << 31) return set_error(TQ_ERR_UNSUPPORTED, "attention: too many rows in one call");
     if (p.splits > 1) slots = units * p.rows * p.splits;

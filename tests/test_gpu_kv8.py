@@ -647,6 +647,24 @@ def test_one_head_over_many_workgroups(D, lens):
             check(dense[b], want.double(), tol.double(), q.dtype, f"16-bit, sequence {b}")
 
 
+@pytest.mark.parametrize("D,nq,T,window", [(64, 512, 4100, 0), (96, 512, 4100, 0), (128, 512, 4100, 0), (128, 300, 9000, 0),
+                                           (128, 770, 3000, 0), (256, 300, 3000, 0), (128, 1030, 4100, 2500), (64, 40, 9000, 0)])
+def test_chunks_in_parts(D, nq, T, window):
+    """Prompt chunks whose tiles go to several workgroups, in tall and low row tiles: some queries of each against float64."""
+    from turboquant_amd import kv8_attention, window_attention
+    H, hq, block, dtype = 8, 32, 32, torch.bfloat16
+    k, v = rand(99, 1, H, T, D, dtype=dtype), rand(100, 1, H, T, D, dtype=dtype, scale=2.0)
+    q = rand(101, 1, hq, nq, D, dtype=dtype, scale=1.5)
+    got = kv8_attention(q, store_of(k, "int8", block, T, v), T, window=window or None, sinks=5)
+    dense = window_attention(q, k, v, window or None, 5)
+    ke, ve = exact_tokens(k[0], T, "int8", block), exact_tokens(v[0], T, "int8", block)
+    for i in (0, 31, nq // 2, nq - 1):
+        n = T - nq + i + 1
+        for name, x, kk, vv in (("8-bit", got, ke, ve), ("16-bit", dense, k[0], v[0])):
+            want, tol = attend(q[0, :, i:i + 1], kk[:, :n], vv[:, :n], n, window, 5, weights=dtype)
+            check(x[0, :, i:i + 1], want, tol, dtype, f"{name}, query {i}")
+
+
 @pytest.mark.parametrize("B,H,T,nq", [(1, 2, 300, 1), (1, 2, 6000, 1), (2, 2, 6000, 3), (1, 2, 900, 70), (32, 8, 200, 20)])
 def test_output_over_the_queries(B, H, T, nq):
     """``out`` may be the queries themselves."""
