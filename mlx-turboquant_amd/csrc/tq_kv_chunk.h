@@ -12,7 +12,7 @@
 //
 // Measured: 2048 queries of 32 heads on 8 over 32,768 tokens, head dim 128, bf16,
 // int8: 1028 us, 1.04 PFLOP/s (a large bf16 product reaches 1.22); 8192 queries
-// over 16-bit keys and values, window 1024: 190 us, 0.68 PFLOP/s of what is seen.
+// over 16-bit keys and values, window 1024: 188 us, 0.69 PFLOP/s of what is seen.
 //
 // Scores, transposed: S^T = K q^T. Key row m of a 32-token half tile is token m
 // with bits 2 and 3 swapped, so that lane (column n, half h) holds, register by
