@@ -267,6 +267,7 @@ int check_store(const tq_kv8_store* s) {
     return set_error(TQ_ERR_UNSUPPORTED, "kv8: blocks of %d tokens: use 16, 32 or 64", s->block);
   if (s->kv_dtype != TQ_F16 && s->kv_dtype != TQ_BF16) return set_error(TQ_ERR_UNSUPPORTED, "kv8: keys and values are fp16 or bf16");
   if (s->batch < 0 || s->heads < 1) return set_error(TQ_ERR_INVALID, "kv8: batch %d, heads %d", s->batch, s->heads);
+  if ((int64_t)s->batch * s->heads >= (int64_t)1 << 31) return set_error(TQ_ERR_UNSUPPORTED, "kv8: too many sequences and heads");
   if (s->cap < 0 || s->cap % TILE || s->cap >= (int64_t)1 << 31)
     return set_error(TQ_ERR_INVALID, "kv8: room for %lld tokens: a multiple of 64 below 2^31", (long long)s->cap);
   if (s->batch == 0 || s->cap == 0) return TQ_OK;

@@ -258,6 +258,7 @@ int plan(const tq_kv8_store* s, const tq_kv_attn_desc* d, Params& p, bool& decod
   p.scale = d->scale * 1.44269504088896340736f;
   decode = p.rows <= DEC_ROWS;
   const int64_t heads = (int64_t)p.batch * p.hkv;
+  if (heads >= (int64_t)1 << 31) return set_error(TQ_ERR_UNSUPPORTED, "attention: too many sequences and heads");
   // tiles that a group of rows reads at most, the tail among them
   const auto most_tiles = [&](int64_t rows) {
     int64_t tiles = ((int64_t)d->max_len + TILE - 1) / TILE;

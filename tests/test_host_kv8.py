@@ -250,6 +250,22 @@ def test_c_entry_points_refuse_before_device_work():
     assert lib.tq_window_attention(de(batch=0), None, 0, None) == 0 and lib.tq_window_attention(de(n_q=0), None, 0, None) == 0
 
 
+def test_batches_whose_products_wrap_are_refused():
+    """2^30 sequences of 2^30 heads: products with rows and tiles come to 2^64, which must not pass for 0."""
+    lib = _lib.load()
+    keep, a = _aligned(64)
+    rows, n = _lib.Rows4(a, 0, 0, 0), 2 ** 30
+    d = ctypes.byref(_lib.KVAttnDesc(batch=n, hq=n, hkv=n, d=64, n_q=2048, dtype=0, out_dtype=0, window=0, sinks=0, max_len=1024,
+                                     len_b=None, scale=1.0, q=rows, out=rows, k=rows, v=rows))
+    s = ctypes.byref(_lib.KV8StoreDesc(k_codes=a, v_codes=a, k_scales=a, v_scales=a, k_tail=a, v_tail=a, cap=1024, fmt=0, d=64, block=32,
+                                       kv_dtype=0, batch=n, heads=n))
+    U = _lib.TQ_ERR_UNSUPPORTED
+    assert lib.tq_window_attention(d, a, 1 << 62, None) == U and lib.tq_window_attention_workspace_bytes(d) == 0
+    assert lib.tq_kv8_attention(s, d, a, 1 << 62, None) == U
+    assert lib.tq_kv8_write(s, ctypes.byref(rows), ctypes.byref(rows), None, 0, None, 512, None) == U
+    assert lib.tq_kv8_read(s, None, 512, 0, 512, 0, a, a, None) == U
+
+
 def test_workspace_is_bounded_by_what_a_window_reads():
     lib = _lib.load()
     keep, a = _aligned(64)
